@@ -5,6 +5,7 @@ Sub-modules:
   build       compile the CUDA library in-tree (no GPU needed)
   _lib        ctypes binding of the C ABI (include/hyc_b200.h); raises if the library is missing
   packed      packed-activation records and Python callers of the C ABI
+  rowops      callers of the row operators: counter-based dropout, layer norm of a residual sum, token log probabilities
   operators   drop-in ``EfficientMemory*`` modules / autograd Functions
   synthetic   seeded synthetic inputs shaped like the benchmark configurations
 
@@ -16,7 +17,7 @@ __version__ = "0.1.0"
 
 OPERATOR_MODULES = ("compress_function", "efficient_linear", "efficient_rmsnorm", "efficient_rmsnorm_gemma",
                     "efficient_layernorm", "efficient_silu", "efficient_gelu", "efficient_hadamard",
-                    "efficient_softmax", "efficient_gemm", "efficient_dropout")
+                    "efficient_softmax", "efficient_gemm", "efficient_dropout", "efficient_logprob")
 
 
 def install_as_operators(name: str = "operators"):

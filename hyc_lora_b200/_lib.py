@@ -80,6 +80,53 @@ class HycSparseRows(C.Structure):
     ]
 
 
+class HycDropoutArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("cols", C.c_int64), ("dtype", C.c_int32), ("_pad", C.c_int32),
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("residual", C.c_void_p), ("residual_stride", C.c_int64),
+        ("y", C.c_void_p), ("rng", C.c_void_p), ("p", C.c_double),
+    ]
+
+
+class HycLayerNormArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("cols", C.c_int32), ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("eps", C.c_float),
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("residual", C.c_void_p), ("residual_stride", C.c_int64),
+        ("weight", C.c_void_p), ("bias", C.c_void_p), ("rng", C.c_void_p), ("p", C.c_double),
+        ("y", C.c_void_p), ("z", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+    ]
+
+
+class HycLayerNormBwdArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("cols", C.c_int32), ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("_pad", C.c_int32),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64), ("z", C.c_void_p), ("z_stride", C.c_int64),
+        ("dz", C.c_void_p), ("dz_stride", C.c_int64), ("weight", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+        ("rng", C.c_void_p), ("p", C.c_double),
+        ("dresidual", C.c_void_p), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("partials", C.c_void_p),
+    ]
+
+
+class HycLogprobArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("rows", C.c_int64), ("row_stride", C.c_int64), ("batch_stride", C.c_int64), ("seq", C.c_int64),
+        ("vocab", C.c_int32), ("dtype", C.c_int32), ("targets", C.c_void_p), ("ignore_index", C.c_int64),
+        ("top", C.c_int32), ("_pad", C.c_int32),
+        ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("stats", C.c_void_p), ("top_logprob", C.c_void_p), ("top_index", C.c_void_p),
+    ]
+
+
+class HycLogprobBwdArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("rows", C.c_int64), ("row_stride", C.c_int64), ("batch_stride", C.c_int64), ("seq", C.c_int64),
+        ("vocab", C.c_int32), ("dtype", C.c_int32), ("targets", C.c_void_p), ("ignore_index", C.c_int64),
+        ("stats", C.c_void_p), ("entropy", C.c_void_p), ("d_logprob", C.c_void_p), ("d_entropy", C.c_void_p), ("d_top", C.c_void_p),
+        ("top_index", C.c_void_p), ("top", C.c_int32), ("_pad", C.c_int32), ("grad", C.c_void_p),
+    ]
+
+
 # every symbol include/hyc_b200.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "hyc_strerror": (C.c_char_p, [C.c_int]),
@@ -113,6 +160,13 @@ SYMBOLS = {
     "hyc_nf4_dequant": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     "hyc_rope": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                            C.c_int32, C.c_void_p]),
+    "hyc_rng_take": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "hyc_dropout": (C.c_int, [C.POINTER(HycDropoutArgs), C.c_void_p]),
+    "hyc_layer_norm": (C.c_int, [C.POINTER(HycLayerNormArgs), C.c_void_p]),
+    "hyc_layer_norm_bwd_scratch_floats": (C.c_int64, [C.c_int64, C.c_int32]),
+    "hyc_layer_norm_bwd": (C.c_int, [C.POINTER(HycLayerNormBwdArgs), C.c_void_p]),
+    "hyc_token_logprobs": (C.c_int, [C.POINTER(HycLogprobArgs), C.c_void_p]),
+    "hyc_token_logprobs_bwd": (C.c_int, [C.POINTER(HycLogprobBwdArgs), C.c_void_p]),
     "hyc_select_channels_static_max_cols": (C.c_int, []),
     "hyc_select_channels_noalloc": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
 }

@@ -227,6 +227,7 @@ const char* hyc_strerror(int code) {
     case HYC_ERR_CAPACITY: return "size exceeds a stated maximum";
     case HYC_ERR_CUDA: return "CUDA runtime error";
     case HYC_ERR_SMEM: return "row too large for shared-memory staging";
+    case HYC_ERR_VALUE: return "a scalar argument is out of its range";
     default: return "unknown error code";
   }
 }

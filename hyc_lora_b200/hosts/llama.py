@@ -31,6 +31,7 @@ class DecoderConfig:
     lora_alpha: float = 16.0
     base_quant: str = "nf4"
     dtype: torch.dtype = torch.bfloat16
+    fused_loss: bool = False       # loss straight from the logits in their own dtype (operators/efficient_logprob.py)
 
     @staticmethod
     def llama2_7b(**kw):
@@ -204,11 +205,29 @@ class DecoderLM(nn.Module):
         self.norm = LlamaRMSNorm(c.hidden, c.eps, device)
         self.lm_head = FrozenLinear(c.hidden, c.vocab, "bf16", device=device, generator=gen, dtype=c.dtype)
 
-    def forward(self, ids):
+    def logits(self, ids):
         x = self.embed_tokens(ids)
         # the first activation has no trainable producer; it must require grad for the LoRA chain rule
         x = x.requires_grad_(True) if not x.requires_grad else x
         for layer in self.layers:
             x = layer(x)
-        logits = self.lm_head(self.norm(x))
+        return self.lm_head(self.norm(x))
+
+    def _next(self, ids):
+        # every row of the logits keeps its place; the last position has no next token
+        return F.pad(ids[:, 1:], (0, 1), value=-100)
+
+    @torch.no_grad()
+    def score(self, ids, entropy: bool = False, top: int = 0):
+        """Log probability of every token after the first (``logprob[:, t]`` is that of ``ids[:, t + 1]``, 0 at the end), with
+        the entropy of the model's distribution and its ``top`` alternatives at every position: a
+        :class:`~hyc_lora_b200.rowops.TokenLogprobs`."""
+        from ..rowops import token_logprobs
+        return token_logprobs(self.logits(ids), self._next(ids), entropy=entropy, top=top)
+
+    def forward(self, ids):
+        logits = self.logits(ids)
+        if self.config.fused_loss:
+            from ..operators.efficient_logprob import token_cross_entropy
+            return token_cross_entropy(logits, self._next(ids))
         return F.cross_entropy(logits[:, :-1].reshape(-1, logits.shape[-1]).float(), ids[:, 1:].reshape(-1))

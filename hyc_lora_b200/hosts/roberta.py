@@ -3,7 +3,9 @@
 Swap points as in the reference's model file (models/modeling_roberta.py:55, 130, 239-279,
 303, 376, 391): ``gemm1`` / ``gemm2`` (class ``RobertaGEMM``), ``softmax`` (``nn.Softmax``),
 ``dropout`` (``nn.Dropout``), ``LayerNorm`` modules, ``intermediate_act_fn`` (class name contains
-"GELU").  LoRA adapters sit on the projections named in ``lora_targets``."""
+"GELU").  With ``hidden_dropout`` each block end is dropout, residual and LayerNorm in one kernel
+(``EfficientMemoryDropoutAddLayerNorm``, which keeps its sum uncompressed) and the embeddings pass a
+counter-based dropout.  LoRA adapters sit on the projections named in ``lora_targets``."""
 from __future__ import annotations
 
 import math
@@ -30,6 +32,7 @@ class EncoderConfig:
     lora_alpha: float = 16.0
     lora_targets: tuple = ("query", "value")
     dtype: torch.dtype = torch.float32
+    hidden_dropout: float = 0.0    # dropout of the embeddings and of every sublayer's output, in front of its residual sum
 
 
 class RobertaGEMM(nn.Module):
@@ -88,16 +91,26 @@ class EncoderLayer(nn.Module):
         super().__init__()
         self.attention = SelfAttention(c, device, gen)
         self.attn_out = _Proj(c, c.hidden, c.hidden, "dense" in c.lora_targets, device, gen)
-        self.attn_LayerNorm = nn.LayerNorm(c.hidden, eps=c.eps, device=device, dtype=c.dtype)
+        self.joined = c.hidden_dropout > 0.0
+        self.attn_LayerNorm = self._norm(c, device)
         self.intermediate = _Proj(c, c.hidden, c.ffn, "dense" in c.lora_targets, device, gen)
         self.intermediate_act_fn = RobertaGELU()
         self.output = _Proj(c, c.ffn, c.hidden, "dense" in c.lora_targets, device, gen)
-        self.out_LayerNorm = nn.LayerNorm(c.hidden, eps=c.eps, device=device, dtype=c.dtype)
+        self.out_LayerNorm = self._norm(c, device)
         for ln in (self.attn_LayerNorm, self.out_LayerNorm):
             ln.weight.requires_grad_(False)
             ln.bias.requires_grad_(False)
 
+    def _norm(self, c, device):
+        if not self.joined:
+            return nn.LayerNorm(c.hidden, eps=c.eps, device=device, dtype=c.dtype)
+        from ..operators.efficient_layernorm import EfficientMemoryDropoutAddLayerNorm
+        return EfficientMemoryDropoutAddLayerNorm(c.hidden, p=c.hidden_dropout, eps=c.eps, device=device, dtype=c.dtype)
+
     def forward(self, x):
+        if self.joined:
+            x = self.attn_LayerNorm(self.attn_out(self.attention(x)), x)
+            return self.out_LayerNorm(self.output(self.intermediate_act_fn(self.intermediate(x))), x)
         x = self.attn_LayerNorm(self.attn_out(self.attention(x)) + x)
         return self.out_LayerNorm(self.output(self.intermediate_act_fn(self.intermediate(x))) + x)
 
@@ -120,6 +133,10 @@ class EncoderClassifier(nn.Module):
         self.emb_LayerNorm = nn.LayerNorm(c.hidden, eps=c.eps, device=device, dtype=c.dtype)
         self.emb_LayerNorm.weight.requires_grad_(False)
         self.emb_LayerNorm.bias.requires_grad_(False)
+        self.emb_dropout = None
+        if c.hidden_dropout > 0.0:
+            from ..operators.efficient_dropout import EfficientMemoryCounterDropout
+            self.emb_dropout = EfficientMemoryCounterDropout(c.hidden_dropout, device=device)
         self.layers = nn.ModuleList(EncoderLayer(c, device, gen) for _ in range(c.layers))
         # the head trains, as in the reference (its dense layer is renamed so LoRA skips it)
         self.class_intermediate = nn.Linear(c.hidden, c.hidden, device=device, dtype=c.dtype)
@@ -133,7 +150,10 @@ class EncoderClassifier(nn.Module):
     def forward(self, ids, labels):
         s = ids.shape[1]
         x = self.word(ids) + self.pos(torch.arange(2, s + 2, device=ids.device))
-        x = self.emb_LayerNorm(x).requires_grad_(True)
+        x = self.emb_LayerNorm(x)
+        if self.emb_dropout is not None:
+            x = self.emb_dropout(x)
+        x = x.requires_grad_(True)
         for layer in self.layers:
             x = layer(x)
         logits = self.out_proj(torch.tanh(self.class_intermediate(x[:, 0])))

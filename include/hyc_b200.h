@@ -39,7 +39,8 @@ typedef enum {
   HYC_ERR_ALIGN = -6,       /* a pointer or stride is not 16-byte aligned         */
   HYC_ERR_CAPACITY = -7,    /* a size exceeds a stated maximum                    */
   HYC_ERR_CUDA = -8,        /* a CUDA runtime call failed (see hyc_last_cuda_error) */
-  HYC_ERR_SMEM = -9         /* the row does not fit the shared-memory staging     */
+  HYC_ERR_SMEM = -9,        /* the row does not fit the shared-memory staging     */
+  HYC_ERR_VALUE = -10       /* a scalar argument is out of its range              */
 } hyc_status;
 
 typedef enum { HYC_F32 = 0, HYC_BF16 = 1 } hyc_dtype;
@@ -299,6 +300,142 @@ int hyc_nf4_dequant(const void* codes, const float* absmax, const float* codeboo
  * Host-model plumbing, not part of the compression path. */
 int hyc_rope(void* q, void* k, const float* cos_sin, int64_t tokens, int32_t seq, int32_t heads_q, int32_t heads_k,
              int32_t head_dim, int32_t inverse, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Row operators of the training step around the compressed sites.  They keep nothing of the tensor's size beyond
+ * what their formulas need: no dropout mask, no fp32 copy of the logits.  (No counterpart among the reference's
+ * kernels: it regenerates its dropout mask from a seed with tensor ops, operators/efficient_dropout.py:7-28, and takes
+ * the loss from the host model, models/modeling_llama.py.)  Rows are `cols` contiguous elements, row t starting at
+ * t * stride elements; strides are >= 0, outputs are contiguous.  No alignment beyond an element's own size is asked
+ * for.  Outputs may not overlap inputs.
+ *
+ * Random words: element i (row-major, i = row * cols + column) of a dropout takes word i % 4 of the Philox4x32-10 block
+ * with counter (i / 4, call) under the key `seed`, `rng` = {seed, call} being two int64 in device memory; it is kept
+ * where the word is at least round(p * 2^32).  p in [0, 1] (else HYC_ERR_VALUE); p = 1 keeps nothing. */
+
+/* used = {seed, call}, then call += 1 in `state` (atomically: calls on several streams take different numbers).
+ * Capturable: every replay of a recorded graph takes new numbers. */
+int hyc_rng_take(int64_t* state, int64_t* used, void* stream);
+
+/* y = residual + (kept ? x / (1 - p) : 0), in fp32, rounded once; residual may be NULL.  What is dropped is selected
+ * away: infinities and NaN there do not reach y.  The backward pass is the same call on the gradient with residual =
+ * NULL and the same rng. */
+typedef struct {
+  int64_t rows, cols;
+  int32_t dtype;           /* hyc_dtype of x, residual, y */
+  int32_t _pad;
+  const void* x;
+  int64_t x_stride;
+  const void* residual;
+  int64_t residual_stride;
+  void* y;                 /* [rows, cols] */
+  const int64_t* rng;
+  double p;
+} hyc_dropout_args;
+int hyc_dropout(const hyc_dropout_args* args, void* stream);
+
+/* z = residual + dropout(x), y = layer norm of z (computed from the unrounded z).  residual, weight, bias and z may be
+ * NULL; rng is read where p > 0.  1 <= cols <= 16384 (HYC_ERR_CAPACITY above).  mean and rstd: fp32 [rows]. */
+typedef struct {
+  int64_t rows;
+  int32_t cols;
+  int32_t dtype;           /* hyc_dtype of x, residual, y, z */
+  int32_t param_dtype;     /* hyc_dtype of weight, bias */
+  float eps;
+  const void* x;
+  int64_t x_stride;
+  const void* residual;
+  int64_t residual_stride;
+  const void* weight;
+  const void* bias;
+  const int64_t* rng;
+  double p;
+  void* y;
+  void* z;
+  float* mean;
+  float* rstd;
+} hyc_layer_norm_args;
+int hyc_layer_norm(const hyc_layer_norm_args* args, void* stream);
+
+/* Its backward pass.  z: the sum as the forward pass stored it (x itself where there was neither residual nor
+ * dropout); dz: a gradient that reaches z past the norm, or NULL.  dresidual = gradient of z; dx = that through the
+ * dropout, needed where p > 0 (where p = 0 it equals dresidual and is not written).  dweight and dbias: [cols] of
+ * param_dtype, NULL where not wanted; summed over the rows in fp32 in a fixed order, rounded once.  `partials`:
+ * 16-byte aligned scratch of hyc_layer_norm_bwd_scratch_floats(rows, cols) floats, needed with dweight or dbias. */
+typedef struct {
+  int64_t rows;
+  int32_t cols;
+  int32_t dtype;
+  int32_t param_dtype;
+  int32_t _pad;
+  const void* dy;
+  int64_t dy_stride;
+  const void* z;
+  int64_t z_stride;
+  const void* dz;
+  int64_t dz_stride;
+  const void* weight;
+  const float* mean;
+  const float* rstd;
+  const int64_t* rng;
+  double p;
+  void* dresidual;
+  void* dx;
+  void* dweight;
+  void* dbias;
+  float* partials;
+} hyc_layer_norm_bwd_args;
+int64_t hyc_layer_norm_bwd_scratch_floats(int64_t rows, int32_t cols);
+int hyc_layer_norm_bwd(const hyc_layer_norm_bwd_args* args, void* stream);
+
+/* Rows of logits -> log probability of each row's target, entropy, the `top` best tokens (largest logit first, the
+ * lower index among equals, a NaN above +inf) with their log probabilities, and stats [rows, 2] = (largest logit m,
+ * log of the sum of exp(x - m)) for the backward pass.  Row t starts at (t / seq) * batch_stride + (t % seq) *
+ * row_stride elements.  targets, entropy, top_* may be NULL (top = 0).  1 <= vocab <= 262144, top <= min(32, vocab).
+ *   - target == ignore_index: logprob 0.  Such a row is not read where neither entropy nor top is asked for; its stats
+ *     are then (-inf, 0).  Any other target outside [0, vocab): logprob NaN.
+ *   - a row whose every logit is -inf: logprob -inf, entropy 0, alternatives the lowest indices at -inf, stats (-inf, 0).
+ *   - a row that holds a NaN or +inf: logprob, entropy and alternatives' log probabilities are NaN. */
+typedef struct {
+  const void* logits;
+  int64_t rows, row_stride, batch_stride, seq;
+  int32_t vocab;
+  int32_t dtype;
+  const int64_t* targets;
+  int64_t ignore_index;
+  int32_t top;
+  int32_t _pad;
+  float* logprob;          /* [rows], with targets */
+  float* entropy;          /* [rows] or NULL */
+  float* stats;            /* [rows, 2], 8-byte aligned */
+  float* top_logprob;      /* [rows, top] */
+  int64_t* top_index;      /* [rows, top] */
+} hyc_logprob_args;
+int hyc_token_logprobs(const hyc_logprob_args* args, void* stream);
+
+/* grad [rows, vocab] (dtype of the logits, rounded once) of what arrives for the log probabilities of the targets
+ * (d_logprob), for the entropies (d_entropy, with the entropies themselves) and for the log probabilities of the
+ * alternatives (d_top, with top_index; an index may repeat or equal the target); each may be NULL.  What arrives for an
+ * ignored row's target counts as 0; rows of stats (-inf, ...) get zeros; a target outside the vocabulary that counts
+ * makes its row NaN; alternatives outside the vocabulary take part in the sum only. */
+typedef struct {
+  const void* logits;
+  int64_t rows, row_stride, batch_stride, seq;
+  int32_t vocab;
+  int32_t dtype;
+  const int64_t* targets;
+  int64_t ignore_index;
+  const float* stats;
+  const float* entropy;
+  const float* d_logprob;
+  const float* d_entropy;
+  const float* d_top;      /* [rows, top] */
+  const int64_t* top_index;
+  int32_t top;
+  int32_t _pad;
+  void* grad;
+} hyc_logprob_bwd_args;
+int hyc_token_logprobs_bwd(const hyc_logprob_bwd_args* args, void* stream);
 
 /* Channel selection for callers that cannot allocate device memory.  (No counterpart in the
  * reference; added for hosts that own no device allocator -- a foreign-language binding that
