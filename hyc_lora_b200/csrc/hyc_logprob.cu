@@ -157,9 +157,9 @@ __global__ void __launch_bounds__(256) logprob_bwd_kernel(const LogprobBwdArgs a
 constexpr int kLpMaxVocab = 262144, kLpMaxTop = 32;
 
 static int check_logprob(int64_t rows, int32_t vocab, int32_t dtype, int64_t seq, int64_t row_stride, int64_t batch_stride, int32_t top) {
-  if (rows < 0 || rows > (1LL << 40) || vocab < 1 || seq < 1 || row_stride < 0 || batch_stride < 0) return HYC_ERR_SHAPE;
+  if (rows < 0 || vocab < 1 || seq < 1 || row_stride < 0 || batch_stride < 0) return HYC_ERR_SHAPE;
   if (top < 0 || top > vocab) return HYC_ERR_SHAPE;
-  if (vocab > kLpMaxVocab || top > kLpMaxTop) return HYC_ERR_CAPACITY;
+  if (vocab > kLpMaxVocab || top > kLpMaxTop || rows > 0x7fffffffLL) return HYC_ERR_CAPACITY;
   if (dtype != HYC_F32 && dtype != HYC_BF16) return HYC_ERR_DTYPE;
   return HYC_OK;
 }

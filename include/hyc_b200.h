@@ -335,7 +335,7 @@ typedef struct {
 int hyc_dropout(const hyc_dropout_args* args, void* stream);
 
 /* z = residual + dropout(x), y = layer norm of z (computed from the unrounded z).  residual, weight, bias and z may be
- * NULL; rng is read where p > 0.  1 <= cols <= 16384 (HYC_ERR_CAPACITY above).  mean and rstd: fp32 [rows]. */
+ * NULL; rng is read where p > 0.  1 <= cols <= 16384 and rows < 2^31 (HYC_ERR_CAPACITY above).  mean and rstd: fp32 [rows]. */
 typedef struct {
   int64_t rows;
   int32_t cols;
@@ -391,7 +391,8 @@ int hyc_layer_norm_bwd(const hyc_layer_norm_bwd_args* args, void* stream);
 /* Rows of logits -> log probability of each row's target, entropy, the `top` best tokens (largest logit first, the
  * lower index among equals, a NaN above +inf) with their log probabilities, and stats [rows, 2] = (largest logit m,
  * log of the sum of exp(x - m)) for the backward pass.  Row t starts at (t / seq) * batch_stride + (t % seq) *
- * row_stride elements.  targets, entropy, top_* may be NULL (top = 0).  1 <= vocab <= 262144, top <= min(32, vocab).
+ * row_stride elements.  targets, entropy, top_* may be NULL (top = 0).  1 <= vocab <= 262144, top <= min(32, vocab),
+ * rows < 2^31.
  *   - target == ignore_index: logprob 0.  Such a row is not read where neither entropy nor top is asked for; its stats
  *     are then (-inf, 0).  Any other target outside [0, vocab): logprob NaN.
  *   - a row whose every logit is -inf: logprob -inf, entropy 0, alternatives the lowest indices at -inf, stats (-inf, 0).

@@ -107,14 +107,14 @@ def _norm_bwd(lib, **kw):
 def test_layer_norm_refusals(lib):
     assert lib.lib.hyc_layer_norm(None, None) == -1 and lib.lib.hyc_layer_norm_bwd(None, None) == -1
     for bad, code in (({"x": None}, -1), ({"y": None}, -1), ({"mean": None}, -1), ({"rstd": None}, -1), ({"p": 0.5}, -1),
-                      ({"rows": -1}, -2), ({"cols": 0}, -2), ({"cols": -5}, -2), ({"x_stride": -1}, -2), ({"cols": 16385}, -7),
+                      ({"rows": -1}, -2), ({"cols": 0}, -2), ({"cols": -5}, -2), ({"x_stride": -1}, -2), ({"cols": 16385}, -7), ({"rows": 2 ** 31}, -7),
                       ({"dtype": 3}, -4), ({"param_dtype": 3}, -4), ({"x": 0x1001}, -6), ({"z": 0x1001}, -6), ({"weight": 0x1002}, -6),
                       ({"bias": 0x1002}, -6), ({"mean": 0x3002}, -6), ({"p": 0.5, "rng": 0x1004}, -6), ({"p": -1.0}, -10),
                       ({"p": float("nan")}, -10)):
         assert _norm(lib, **bad) == code, bad
     for bad, code in (({"dy": None}, -1), ({"z": None}, -1), ({"mean": None}, -1), ({"dresidual": None}, -1),
                       ({"p": 0.5, "rng": 0x1000}, -1), ({"p": 0.5, "dx": 0x1000}, -1), ({"dweight": 0x1000}, -1), ({"dbias": 0x1000}, -1),
-                      ({"dy_stride": -1}, -2), ({"cols": 0}, -2), ({"cols": 16385}, -7), ({"dtype": 3}, -4), ({"dz": 0x1001}, -6),
+                      ({"dy_stride": -1}, -2), ({"cols": 0}, -2), ({"cols": 16385}, -7), ({"rows": 2 ** 31}, -7), ({"dtype": 3}, -4), ({"dz": 0x1001}, -6),
                       ({"dweight": 0x1002, "partials": 0x1000}, -6), ({"dweight": 0x1000, "partials": 0x1008}, -6), ({"p": 2.0}, -10)):
         assert _norm_bwd(lib, **bad) == code, bad
     assert _norm(lib, rows=0, x=None, y=None, mean=None, rstd=None) == 0
@@ -146,7 +146,7 @@ def _logprob_bwd(lib, **kw):
 def test_logprob_refusals(lib):
     assert lib.lib.hyc_token_logprobs(None, None) == -1 and lib.lib.hyc_token_logprobs_bwd(None, None) == -1
     common = (({"logits": None}, -1), ({"stats": None}, -1), ({"rows": -1}, -2), ({"vocab": 0}, -2), ({"seq": 0}, -2),
-              ({"row_stride": -1}, -2), ({"batch_stride": -1}, -2), ({"top": -1}, -2), ({"vocab": 262145}, -7), ({"dtype": 2}, -4),
+              ({"row_stride": -1}, -2), ({"batch_stride": -1}, -2), ({"top": -1}, -2), ({"vocab": 262145}, -7), ({"rows": 2 ** 31}, -7), ({"dtype": 2}, -4),
               ({"logits": 0x1001}, -6), ({"targets": 0x2004}, -6), ({"stats": 0x4004}, -6))
     for bad, code in common + (({"logprob": None}, -1), ({"top": 5}, -1), ({"top": 101}, -2), ({"top": 33}, -7),
                                ({"top": 5, "top_index": 0x1004, "top_logprob": 0x1000}, -6), ({"entropy": 0x1002}, -6)):
