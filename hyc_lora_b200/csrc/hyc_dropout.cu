@@ -29,72 +29,128 @@ __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { retu
 // Any addresses and strides.  One thread: the four elements of one counter block.
 template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs a) {
-  const Philox gen = Philox::load(a.rng);
+  Philox gen = Philox::load(a.rng);
   const long long n = a.rows * a.cols, blocks = (n + 3) >> 2;
   const T* x = static_cast<const T*>(a.x);
   const T* res = static_cast<const T*>(a.residual);
   T* y = static_cast<T*>(a.y);
   for (long long b = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; b < blocks;
        b += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const uint4 w4 = gen.block(static_cast<unsigned long long>(b));
+    const uint4 w4 = gen.at(static_cast<unsigned long long>(b));
     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
     long long row = 4 * b / a.cols, col = 4 * b - row * a.cols;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (4 * b + e >= n) break;
       const float base = RES ? to_float<T>(res[row * a.residual_stride + col]) : 0.f;
-      const float v = to_float<T>(x[row * a.x_stride + col]);
+      const float v = a.rate.none ? 0.f : to_float<T>(x[row * a.x_stride + col]);
       y[4 * b + e] = T(a.rate.keep(w[e]) ? fmaf(v, a.rate.scale, base) : base);
       if (++col == a.cols) { col = 0; ++row; }
     }
   }
 }
 
-// One flat run of elements at 16-byte aligned addresses.  A thread takes kDropUnits pieces of eight elements (two counter
-// blocks each) that lie a CTA's width apart, all loads before the first use.  What bounds it is DRAM as long as the ten
-// rounds of the generator (about 11 instructions per element) stay under the issue slots that the traffic leaves: 22 per
-// element for bf16 without a residual.
-constexpr int kDropUnits = 2;
+// One flat run of elements at 16-byte aligned addresses.  Persistent: a CTA takes tiles of U * 256 pieces of 16 bytes and has
+// the next tile's loads in flight while it draws this tile's words.  Without a residual and in bf16 the generator's
+// multiplications (see hyc_philox.cuh) bound it next to DRAM, else DRAM alone.  Many words per turn keep the multiplier fed:
+// 8192 x 11008 bf16 takes 74 us with U = 8, 77 with 6, 80 with 4, 83 with 2 and 79 with 12 (DRAM alone: 56).
 
-template <typename T, bool RES>
-__global__ void __launch_bounds__(256) dropout_flat_kernel(const DropoutArgs a) {
-  const Philox gen = Philox::load(a.rng);
-  const long long units = a.cols >> 3;
-  const T* x = static_cast<const T*>(a.x);
-  const T* res = static_cast<const T*>(a.residual);
-  T* y = static_cast<T*>(a.y);
-  const long long first = static_cast<long long>(blockIdx.x) * (256 * kDropUnits) + threadIdx.x;
-  float v[kDropUnits][8], r[kDropUnits][8];
+// eight bf16 values as fp32; both halves by byte permutes and masks, which leave the multiplier's pipe to the generator
+__device__ __forceinline__ void piece_to_floats(const uint4& w, float (&f)[8]) {
+  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int u = 0; u < kDropUnits; ++u) {
-    const long long unit = first + u * 256;
-    if (unit < units) {
-      load8_stream(x + unit * 8, v[u]);
-      if (RES) load8_stream(res + unit * 8, r[u]);
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(__byte_perm(q[i], 0, 0x1044));
+    f[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void piece_to_floats(const uint4& w, float (&f)[4]) {
+  f[0] = __uint_as_float(w.x); f[1] = __uint_as_float(w.y); f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ uint4 floats_to_piece(const float (&f)[8]) { return pack_bf16x8(f); }
+__device__ __forceinline__ uint4 floats_to_piece(const float (&f)[4]) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+
+template <typename T, bool RES, int U>
+struct DropTile {
+  static constexpr int kPiece = 16 / sizeof(T), kBlocks = kPiece / 4;
+  uint4 x[U], r[U];
+
+  __device__ __forceinline__ void load(const DropoutArgs& a, long long first) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u] = load16_stream(static_cast<const uint4*>(a.x) + first + u * 256);
+      if (RES) r[u] = load16_stream(static_cast<const uint4*>(a.residual) + first + u * 256);
     }
   }
+  __device__ __forceinline__ static uint4 piece(const DropoutArgs& a, const Philox& gen, const uint4& xp, const uint4& rp, uint32_t block) {
+    float f[kPiece], base[kPiece];
+    piece_to_floats(xp, f);
+    if (RES) piece_to_floats(rp, base);
 #pragma unroll
-  for (int u = 0; u < kDropUnits; ++u) {
-    const long long unit = first + u * 256;
-    if (unit < units) {
-      const uint4 lo = gen.block(2ull * unit), hi = gen.block(2ull * unit + 1);
-      const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    for (int q = 0; q < kBlocks; ++q) {
+      const uint4 w = gen.block(block + q);
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float base = RES ? r[u][e] : 0.f;
-        v[u][e] = a.rate.keep(w[e]) ? fmaf(v[u][e], a.rate.scale, base) : base;
+      for (int e = 0; e < 4; ++e) {
+        const float b = RES ? base[4 * q + e] : 0.f;
+        f[4 * q + e] = a.rate.keep(words[e]) ? fmaf(f[4 * q + e], a.rate.scale, b) : b;
       }
-      store8<T>(y + unit * 8, 0, v[u]);
     }
+    return floats_to_piece(f);
   }
-  // the last elements, fewer than eight
-  const long long e = units * 8 + threadIdx.x;
-  if (blockIdx.x == 0 && e < a.cols) {
-    const uint4 w = gen.block(static_cast<unsigned long long>(e >> 2));
+  __device__ __forceinline__ void finish(const DropoutArgs& a, Philox& gen, long long first) const {
+    const unsigned long long block = static_cast<unsigned long long>(first) * kBlocks;
+    if (static_cast<uint32_t>(block >> 32) != gen.upper) gen.prepare(static_cast<uint32_t>(block >> 32));
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      static_cast<uint4*>(a.y)[first + u * 256] = piece(a, gen, x[u], r[u], static_cast<uint32_t>(block) + u * 256 * kBlocks);
+  }
+};
+
+template <typename T, bool RES, int U>
+__global__ void __launch_bounds__(256, 1) dropout_flat_kernel(const DropoutArgs a) {
+  using Tile = DropTile<T, RES, U>;
+  constexpr int kTile = 256 * U, kBlocks = Tile::kBlocks;
+  Philox gen = Philox::load(a.rng);
+  const long long pieces = a.cols / Tile::kPiece, tiles = pieces / kTile;    // a tile's counters share their upper half
+  if (!a.rate.none) {
+    Tile one, two;
+    long long tile = blockIdx.x;
+    if (tile < tiles) one.load(a, tile * kTile + threadIdx.x);
+    while (tile < tiles) {
+      long long next = tile + gridDim.x;
+      if (next < tiles) two.load(a, next * kTile + threadIdx.x);
+      one.finish(a, gen, tile * kTile + threadIdx.x);
+      if (next >= tiles) break;
+      tile = next;
+      next += gridDim.x;
+      if (next < tiles) one.load(a, next * kTile + threadIdx.x);
+      two.finish(a, gen, tile * kTile + threadIdx.x);
+      tile = next;
+    }
+  } else {
+    for (long long p = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; p < tiles * kTile; p += static_cast<long long>(gridDim.x) * 256)
+      static_cast<uint4*>(a.y)[p] = RES ? static_cast<const uint4*>(a.residual)[p] : make_uint4(0, 0, 0, 0);
+  }
+  // the pieces behind the last whole tile, and the elements behind the last piece
+  if (blockIdx.x != tiles % gridDim.x) return;
+  for (long long p = tiles * kTile + threadIdx.x; p < pieces; p += 256) {
+    const unsigned long long block = static_cast<unsigned long long>(p) * kBlocks;
+    if (static_cast<uint32_t>(block >> 32) != gen.upper) gen.prepare(static_cast<uint32_t>(block >> 32));
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    static_cast<uint4*>(a.y)[p] = Tile::piece(a, gen, a.rate.none ? zero : static_cast<const uint4*>(a.x)[p],
+                                              RES ? static_cast<const uint4*>(a.residual)[p] : zero, static_cast<uint32_t>(block));
+  }
+  const long long e = pieces * Tile::kPiece + threadIdx.x;
+  if (e < a.cols) {
+    const uint4 w = gen.at(static_cast<unsigned long long>(e >> 2));
     const int lane = static_cast<int>(e & 3);
-    const float base = RES ? to_float<T>(res[e]) : 0.f;
+    const float base = RES ? to_float<T>(static_cast<const T*>(a.residual)[e]) : 0.f;
     const bool keep = a.rate.keep(lane == 0 ? w.x : lane == 1 ? w.y : lane == 2 ? w.z : w.w);
-    y[e] = T(keep ? fmaf(to_float<T>(x[e]), a.rate.scale, base) : base);
+    const float last = a.rate.none ? 0.f : to_float<T>(static_cast<const T*>(a.x)[e]);
+    static_cast<T*>(a.y)[e] = T(keep ? fmaf(last, a.rate.scale, base) : base);
   }
 }
 
@@ -103,16 +159,28 @@ __global__ void rng_take_kernel(unsigned long long* state, long long* used) {
   used[1] = static_cast<long long>(atomicAdd(state + 1, 1ull));
 }
 
+template <typename T, bool RES, int U>
+static void run_dropout_flat(const DropoutArgs& a, cudaStream_t stream) {
+  auto kernel = dropout_flat_kernel<T, RES, U>;
+  const long long blocks = a.cols / (256 * U * (16 / sizeof(T))) + 1;
+  kernel<<<resident_grid(kernel, 256, 0, static_cast<int>(blocks < 1 << 20 ? blocks : 1 << 20)), 256, 0, stream>>>(a);
+}
+
 template <typename T>
 static int launch_dropout(const DropoutArgs& a, cudaStream_t stream) {
   const bool flat = a.rows == 1 && aligned16(a.x) && aligned16(a.y) && aligned16(a.residual);
-  const long long per_block = flat ? 256 * 8 * kDropUnits : 1024, blocks = (a.rows * a.cols + per_block - 1) / per_block;
-  if (flat && blocks <= 0x7fffffffLL) {
-    if (a.residual)
-      dropout_flat_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
-    else
-      dropout_flat_kernel<T, false><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+  if (flat) {
+    // small tensors: one piece per thread on as many SMs as there are
+    const bool large = a.cols * static_cast<long long>(sizeof(T)) >= 16LL * 256 * 8 * 4 * sm_count();
+    if (a.residual) {
+      if (large) run_dropout_flat<T, true, 4>(a, stream);
+      else run_dropout_flat<T, true, 1>(a, stream);
+    } else {
+      if (large) run_dropout_flat<T, false, 8>(a, stream);
+      else run_dropout_flat<T, false, 1>(a, stream);
+    }
   } else {
+    const long long blocks = (a.rows * a.cols + 1023) / 1024;
     const int grid = static_cast<int>(blocks < 1 << 30 ? blocks : 1 << 30);
     if (a.residual)
       dropout_any_kernel<T, true><<<grid, 256, 0, stream>>>(a);

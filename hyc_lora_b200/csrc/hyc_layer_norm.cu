@@ -39,94 +39,226 @@ struct LnBwdArgs {
 
 // ---------------------------------------------------------------- how a row is held
 // A row belongs to G threads (a warp, or a group of warps with a named barrier of its own) that keep it in registers: one read
-// of the row, statistics in two exact passes over registers, one write.  VEC: thread t owns the 8-element pieces t, t + G, ...
-// (16-byte accesses; every address of every row 16-byte aligned).  Otherwise it owns the elements t, t + G, ... (coalesced
-// accesses of single elements, for odd widths and unaligned tensors).
+// of the row, statistics in two exact passes over registers, one write.  A thread has VPT slots of eight elements.
+//   VEC 1  16-byte pieces (8 bf16 or 4 fp32): thread t owns the pieces t, t + G, ...; every address of every row is 16-byte
+//          aligned and a row is a multiple of eight elements;
+//   VEC 2  the same where the row fills its threads' slots exactly: no bounds are left to test;
+//   VEC 0  the elements t, t + G, ... (coalesced accesses of single elements, for odd widths and unaligned tensors).
 
-template <typename T>
-__device__ __forceinline__ float ln_load(const void* p, long long i) { return static_cast<const T*>(p)[i]; }
-template <typename T>
-__device__ __forceinline__ void ln_store(void* p, long long i, float v) { static_cast<T*>(p)[i] = T(v); }
+template <int VEC>
+__device__ __forceinline__ bool ln_in(int c, int cols) { return VEC == 2 || c < cols; }
 
-template <int G, bool VEC>
-__device__ __forceinline__ int ln_col(int t, int v, int j) { return VEC ? (v * G + t) * 8 + j : (v * 8 + j) * G + t; }
+template <typename T, int G, int VEC>
+__device__ __forceinline__ int ln_col(int t, int v, int j) {
+  if (!VEC) return (v * 8 + j) * G + t;
+  return sizeof(T) == 2 ? (v * G + t) * 8 + j : ((2 * v + (j >> 2)) * G + t) * 4 + (j & 3);
+}
 
-// the eight elements of slot v of thread t, `fill` beyond the row's end
-template <typename T, int G, bool VEC>
-__device__ __forceinline__ void ln_get(const void* row, int t, int v, int cols, float (&f)[8]) {
-  if (VEC) {
-    const int c = (v * G + t) * 8;
-    if (c < cols) {
-      load8_stream(static_cast<const T*>(row) + c, f);
-    } else {
+// a 16-byte piece as fp32 pairs, at f
+__device__ __forceinline__ void ln_unpack(const uint4& w, __nv_bfloat16, f32x2* f) {
+  // byte permutes and masks: the multiplier's pipe is left to the generator's products
+  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.f;
+  for (int i = 0; i < 4; ++i) f[i] = f2_make(__uint_as_float(__byte_perm(q[i], 0, 0x1044)), __uint_as_float(q[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void ln_unpack(const uint4& w, float, f32x2* f) {
+  f[0] = f2_make(__uint_as_float(w.x), __uint_as_float(w.y));
+  f[1] = f2_make(__uint_as_float(w.z), __uint_as_float(w.w));
+}
+__device__ __forceinline__ f32x2 f2_both(float v) { return f2_make(v, v); }
+
+// the eight elements of slot v of thread t as four pairs, zero beyond the row's end
+template <typename T, int G, int VEC>
+__device__ __forceinline__ void ln_get(const void* row, int t, int v, int cols, f32x2 (&f)[4]) {
+  if (VEC) {
+    constexpr int kPiece = 16 / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 8 / kPiece; ++h) {
+      const int c = ln_col<T, G, VEC>(t, v, h * kPiece);
+      ln_unpack(ln_in<VEC>(c, cols) ? load16_stream(static_cast<const T*>(row) + c) : make_uint4(0, 0, 0, 0), T(0.f), f + h * (kPiece / 2));
     }
   } else {
+    float e[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int c = (v * 8 + j) * G + t;
-      f[j] = c < cols ? static_cast<float>(static_cast<const T*>(row)[c]) : 0.f;
+      const int c = ln_col<T, G, VEC>(t, v, j);
+      e[j] = c < cols ? static_cast<float>(static_cast<const T*>(row)[c]) : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = f2_make(e[2 * i], e[2 * i + 1]);
   }
 }
 
-template <typename T, int G, bool VEC>
-__device__ __forceinline__ void ln_put(void* row, int t, int v, int cols, const float (&f)[8]) {
+template <typename T, int G, int VEC>
+__device__ __forceinline__ void ln_put(void* row, int t, int v, int cols, const f32x2 (&p)[4]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f2_split(p[i], f[2 * i], f[2 * i + 1]);
   if (VEC) {
-    const int c = (v * G + t) * 8;
-    if (c < cols) store8<T>(static_cast<T*>(row) + c, 0, f);
+    constexpr int kPiece = 16 / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 8 / kPiece; ++h) {
+      const int c = ln_col<T, G, VEC>(t, v, h * kPiece);
+      if (!ln_in<VEC>(c, cols)) continue;
+      uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(row) + c);
+      if (sizeof(T) == 2) *to = pack_bf16x8(f);
+      else *to = make_uint4(__float_as_uint(f[4 * h]), __float_as_uint(f[4 * h + 1]), __float_as_uint(f[4 * h + 2]), __float_as_uint(f[4 * h + 3]));
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int c = (v * 8 + j) * G + t;
+      const int c = ln_col<T, G, VEC>(t, v, j);
       if (c < cols) static_cast<T*>(row)[c] = T(f[j]);
     }
   }
 }
 
 // weight or bias: read again for every row (L1 keeps them), as fp32
-template <int G, bool VEC>
-__device__ __forceinline__ void ln_param(const void* p, bool bf16, int t, int v, int cols, float fill, float (&f)[8]) {
-  if (VEC) {
-    const int c = (v * G + t) * 8;
-    if (p && c < cols) {
-      if (bf16) load8<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(p), c, f);
-      else load8<float>(static_cast<const float*>(p), c, f);
-      return;
-    }
+template <typename T, int G, int VEC>
+__device__ __forceinline__ void ln_param(const void* p, bool bf16, int t, int v, int cols, float fill, f32x2 (&f)[4]) {
+  if (VEC != 2 || !p) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = fill;
+    for (int i = 0; i < 4; ++i) f[i] = f2_both(fill);
+    if (!p) return;
+  }
+  if (VEC) {
+    constexpr int kRun = 16 / sizeof(T);                   // consecutive columns of a thread
+#pragma unroll
+    for (int h = 0; h < 8 / kRun; ++h) {
+      const int c = ln_col<T, G, VEC>(t, v, h * kRun);
+      if (!ln_in<VEC>(c, cols)) continue;
+#pragma unroll
+      for (int q = 0; q < kRun / 4; ++q) {
+        f32x2* to = f + h * (kRun / 2) + q * 2;
+        if (bf16) {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + c + 4 * q));
+          to[0] = f2_make(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u));
+          to[1] = f2_make(__uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+        } else {
+          const float4 w = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + 4 * q));
+          to[0] = f2_make(w.x, w.y);
+          to[1] = f2_make(w.z, w.w);
+        }
+      }
+    }
   } else {
+    float e[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int c = (v * 8 + j) * G + t;
-      f[j] = fill;
-      if (p && c < cols) f[j] = bf16 ? ln_load<__nv_bfloat16>(p, c) : static_cast<const float*>(p)[c];
+      const int c = ln_col<T, G, VEC>(t, v, j);
+      e[j] = fill;
+      if (c < cols) e[j] = bf16 ? static_cast<float>(static_cast<const __nv_bfloat16*>(p)[c]) : static_cast<const float*>(p)[c];
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = f2_make(e[2 * i], e[2 * i + 1]);
   }
 }
 
-// which of the eight elements of a slot are kept; `first` is the index of the row's first element in the tensor
-template <int G, bool VEC>
-__device__ __forceinline__ uint32_t ln_kept(const Philox& gen, const DropRate& rate, unsigned long long first, int t, int v) {
-  uint32_t kept = 0;
-  if (VEC) {                                   // rows of a multiple of eight elements: two whole counter blocks
-    const unsigned long long block = (first + static_cast<unsigned>((v * G + t) * 8)) >> 2;
-    const uint4 lo = gen.block(block), hi = gen.block(block + 1);
-    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+// The same from a table in shared memory that a persistent CTA fills once: fp32, a thread's four columns of a half slot in
+// one 16-byte piece and the pieces of consecutive threads side by side.  Read from L1 for every row instead, the parameters
+// cost the forward pass 250 us against 203 and the backward pass 174 against 145 (32768 x 4096 bf16; half of those reads miss
+// next to the streams).
+template <typename T, int G>
+__device__ __forceinline__ void ln_table_fill(float* table, const void* p, bool bf16, int cols, int slots, float fill) {
+  for (int c = threadIdx.x; c < slots * 8 * G; c += blockDim.x) {
+    float value = fill;
+    if (p && c < cols) value = bf16 ? static_cast<float>(static_cast<const __nv_bfloat16*>(p)[c]) : static_cast<const float*>(p)[c];
+    const int piece = c >> 3;
+    table[sizeof(T) == 4 ? c : ((piece / G * 2 + (c >> 2 & 1)) * G + piece % G) * 4 + (c & 3)] = value;
+  }
+}
+template <int G>
+__device__ __forceinline__ void ln_table_get(const float* table, int t, int v, f32x2 (&f)[4]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) kept |= rate.keep(w[j]) ? 1u << j : 0u;
+  for (int h = 0; h < 2; ++h) {
+    const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(table + ((2 * v + h) * G + t) * 4);
+    f[2 * h] = w.x;
+    f[2 * h + 1] = w.y;
+  }
+}
+
+// base + (kept ? x * scale : 0) of a slot; `first` is the index of the row's first element in the tensor
+template <typename T, int G, int VEC, bool BASE>
+__device__ __forceinline__ void ln_drop(Philox& gen, const DropRate& rate, unsigned long long first, int t, int v, f32x2 (&x)[4],
+                                        const f32x2 (&base)[4]) {
+  uint32_t w[8];
+  if (VEC) {                                   // rows of a multiple of eight elements: two whole counter blocks
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // bf16: the second block follows the first, whose index is even: it has the same upper half
+      const unsigned long long at = (first + static_cast<unsigned>(ln_col<T, G, VEC>(t, v, sizeof(T) == 2 ? 0 : 4 * h))) >> 2;
+      if (sizeof(T) == 4 || h == 0) {
+        if (static_cast<uint32_t>(at >> 32) != gen.upper) gen.prepare(static_cast<uint32_t>(at >> 32));
+      }
+      const uint4 q = gen.block(static_cast<uint32_t>(at) + (sizeof(T) == 2 ? h : 0));
+      w[4 * h] = q.x; w[4 * h + 1] = q.y; w[4 * h + 2] = q.z; w[4 * h + 3] = q.w;
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const unsigned long long element = first + static_cast<unsigned>((v * 8 + j) * G + t);
-      const uint4 w = gen.block(element >> 2);
+      const unsigned long long element = first + static_cast<unsigned>(ln_col<T, G, VEC>(t, v, j));
+      const uint4 q = gen.at(element >> 2);
       const uint32_t lane = static_cast<uint32_t>(element & 3);
-      kept |= rate.keep(lane == 0 ? w.x : lane == 1 ? w.y : lane == 2 ? w.z : w.w) ? 1u << j : 0u;
+      w[j] = lane == 0 ? q.x : lane == 1 ? q.y : lane == 2 ? q.z : q.w;
     }
   }
-  return kept;
+  if (rate.none) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = f2_both(0.f);
+  }
+  const f32x2 scale = f2_both(rate.scale);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi, b0 = 0.f, b1 = 0.f;
+    f2_split(BASE ? f2_fma(x[i], scale, base[i]) : f2_mul(x[i], scale), lo, hi);
+    if (BASE) f2_split(base[i], b0, b1);
+    x[i] = f2_make(rate.keep(w[2 * i]) ? lo : b0, rate.keep(w[2 * i + 1]) ? hi : b1);
+  }
+}
+
+// The rows to come of a group, on their way into shared memory while this one is worked on.  Every thread copies the pieces
+// that it will read itself, so the copies need no barrier: a thread waits for its own (cp.async.wait_group).  One commit per
+// turn, also where there is nothing left to copy, keeps the count.
+template <typename T, int G, int VPT, int VEC, int ARRAYS, int STAGES, int THREADS>
+struct LnRing {
+  static constexpr int kPieces = VPT * 8 * static_cast<int>(sizeof(T)) / 16;
+  static constexpr uint32_t kStageBytes = ARRAYS * kPieces * THREADS * 16u, kBytes = STAGES * kStageBytes;
+  unsigned char* own;
+
+  __device__ __forceinline__ void init(unsigned char* smem) { own = smem + threadIdx.x * 16; }
+  __device__ __forceinline__ unsigned char* slot(int stage, int array, int piece) const {
+    return own + stage * kStageBytes + (array * kPieces + piece) * (THREADS * 16);
+  }
+  __device__ __forceinline__ void copy(int stage, int array, const void* row, int t, int cols) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int c = (i * G + t) * (16 / static_cast<int>(sizeof(T)));
+      if (ln_in<VEC>(c, cols))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slot(stage, array, i))),
+                     "l"(__cvta_generic_to_global(static_cast<const T*>(row) + c))
+                     : "memory");
+    }
+  }
+  __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory"); }
+  __device__ __forceinline__ void get(int stage, int array, int t, int v, int cols, f32x2 (&f)[4]) const {
+    constexpr int kPiece = 16 / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 8 / kPiece; ++h) {
+      const int i = v * (8 / kPiece) + h;
+      const bool in = ln_in<VEC>((i * G + t) * kPiece, cols);
+      ln_unpack(in ? *reinterpret_cast<const uint4*>(slot(stage, array, i)) : make_uint4(0, 0, 0, 0), T(0.f), f + h * (kPiece / 2));
+    }
+  }
+};
+
+// A thread's place in its group, and its group's in the CTA -- the same in every thread of a warp, which a warp-wide
+// reduction lets the compiler know, so that rows' addresses are worked out once per warp, off the multiplier's pipe.
+template <int G, int GROUPS>
+__device__ __forceinline__ int group_thread() { return GROUPS == 1 ? threadIdx.x : threadIdx.x % G; }
+template <int G, int GROUPS>
+__device__ __forceinline__ int group_index() {
+  return GROUPS == 1 ? 0 : static_cast<int>(__reduce_max_sync(0xffffffffu, threadIdx.x / G));
 }
 
 template <int G>
@@ -135,92 +267,82 @@ __device__ __forceinline__ void group_sync() {
   else asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / G), "n"(G) : "memory");
 }
 
-// Sums of N values over the G threads of a group, the same bits in every thread.  `slot` is the group's own, N * 32 floats,
-// and is not used again before the group has met at another barrier.
-template <int G, int N>
-__device__ __forceinline__ void group_sum(float (&v)[N], float* slot) {
+// Sums over the G threads of a group, the same bits in every thread.  `slot` is the group's own (2 * G / 32 floats, 16-byte
+// aligned) and is not used again before the group has met at another barrier.
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float* slot) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  }
-  if (G == 32) return;
-  const int warp = (threadIdx.x % G) >> 5;
-  if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) slot[i * 32 + warp] = v[i];
-  }
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (G == 32) return v;
+  if ((threadIdx.x & 31) == 0) slot[(threadIdx.x % G) >> 5] = v;
   group_sync<G>();
+  float r = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float r = 0.f;
-#pragma unroll
-    for (int w = 0; w < G / 32; ++w) r += slot[i * 32 + w];
-    v[i] = r;
+  for (int w = 0; w < G / 128; ++w) {
+    const float4 p = *reinterpret_cast<const float4*>(slot + 4 * w);
+    r += (p.x + p.y) + (p.z + p.w);
   }
+  return r;
+}
+// two at once: after the first exchange each half of a warp carries one of them
+template <int G>
+__device__ __forceinline__ float2 group_sum2(float v0, float v1, float* slot) {
+  const bool upper = threadIdx.x & 16;
+  float v = (upper ? v1 : v0) + __shfl_xor_sync(0xffffffffu, upper ? v0 : v1, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (G == 32) return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+  if ((threadIdx.x & 15) == 0) slot[((threadIdx.x % G) >> 5) * 2 + (upper ? 1 : 0)] = v;
+  group_sync<G>();
+  float2 r = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < G / 64; ++w) {
+    const float4 p = *reinterpret_cast<const float4*>(slot + 4 * w);
+    r.x += p.x + p.z;
+    r.y += p.y + p.w;
+  }
+  return r;
 }
 
 // ---------------------------------------------------------------- forward
 
-// One row per group of G threads, CTAs of at least 256 threads.  Traffic is what the formula needs; the loads of a whole
-// row are in flight before the first sum, and rows of other groups on the SM cover the two reductions.
-template <typename T, int G, int VPT, bool DROP, bool VEC>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) ln_fwd_kernel(const LnFwdArgs a) {
-  constexpr int kThreads = G < 256 ? 256 : G, kGroups = kThreads / G;
-  __shared__ float slots[kGroups][2][32];
-  const int t = threadIdx.x % G, group = threadIdx.x / G;
-  const long long row = static_cast<long long>(blockIdx.x) * kGroups + group;
-  if (row >= a.rows) return;
-  const void* x = static_cast<const T*>(a.x) + row * a.x_stride;
-  float z[VPT][8];
-#pragma unroll
-  for (int v = 0; v < VPT; ++v) ln_get<T, G, VEC>(x, t, v, a.cols, z[v]);
-  if (a.residual) {
-    const void* res = static_cast<const T*>(a.residual) + row * a.residual_stride;
-    float r[VPT][8];
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) ln_get<T, G, VEC>(res, t, v, a.cols, r[v]);
-    if (DROP) {
-      const Philox gen = Philox::load(a.rng);
-#pragma unroll
-      for (int v = 0; v < VPT; ++v) {
-        const uint32_t kept = ln_kept<G, VEC>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, t, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z[v][j] = kept >> j & 1 ? fmaf(z[v][j], a.rate.scale, r[v][j]) : r[v][j];
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < VPT; ++v)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z[v][j] += r[v][j];
-    }
-  } else if (DROP) {
-    const Philox gen = Philox::load(a.rng);
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      const uint32_t kept = ln_kept<G, VEC>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, t, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) z[v][j] = kept >> j & 1 ? z[v][j] * a.rate.scale : 0.f;
-    }
-  }
-  float s[1] = {0.f};
+// z in registers (where the residual, if any, has been read into r) -> statistics, y, z
+template <typename T, int G, int VPT, bool DROP, int VEC, bool TABLE>
+__device__ __forceinline__ void ln_fwd_row(const LnFwdArgs& a, Philox& gen, long long row, int t, f32x2 (&z)[VPT][4], f32x2 (&r)[VPT][4],
+                                           float* slot, const float* table) {
+  f32x2 s2 = f2_both(0.f);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const float(&p)[8] = z[v];                       // zero beyond the row's end
-    s[0] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-  }
-  group_sum<G, 1>(s, slots[group][0]);
-  const float mean = s[0] / a.cols;
-  float q[1] = {0.f};
+    if (DROP) ln_drop<T, G, VEC, true>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, t, v, z[v], r[v]);
+    else {
 #pragma unroll
-  for (int v = 0; v < VPT; ++v)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float d = z[v][j] - mean;
-      if (ln_col<G, VEC>(t, v, j) < a.cols) q[0] = fmaf(d, d, q[0]);
+      for (int i = 0; i < 4; ++i) z[v][i] = f2_add(z[v][i], r[v][i]);
     }
-  group_sum<G, 1>(q, slots[group][1]);
-  const float rstd = rsqrtf(q[0] / a.cols + a.eps);
+    s2 = f2_add(s2, f2_add(f2_add(z[v][0], z[v][1]), f2_add(z[v][2], z[v][3])));      // zero beyond the row's end
+  }
+  float lo, hi;
+  f2_split(s2, lo, hi);
+  const float mean = group_sum<G>(lo + hi, slot) / a.cols;
+  const f32x2 minus_mean = f2_both(-mean);
+  f32x2 q2 = f2_both(0.f);
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 d = f2_add(z[v][i], minus_mean);
+      if (VEC) {
+        if (ln_in<VEC>(ln_col<T, G, VEC>(t, v, 2 * i), a.cols)) q2 = f2_fma(d, d, q2);   // a piece is in the row or is not
+      } else {
+        f2_split(d, lo, hi);
+        if (ln_col<T, G, VEC>(t, v, 2 * i) >= a.cols) lo = 0.f;
+        if (ln_col<T, G, VEC>(t, v, 2 * i + 1) >= a.cols) hi = 0.f;
+        const f32x2 in = f2_make(lo, hi);
+        q2 = f2_fma(in, in, q2);
+      }
+    }
+  }
+  f2_split(q2, lo, hi);
+  const float rstd = rsqrtf(group_sum<G>(lo + hi, slot + 32) / a.cols + a.eps);
   if (t == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
   void* y = static_cast<T*>(a.y) + row * a.cols;
   if (a.z) {
@@ -228,142 +350,268 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) ln_fwd_kernel(const LnFwdAr
 #pragma unroll
     for (int v = 0; v < VPT; ++v) ln_put<T, G, VEC>(zp, t, v, a.cols, z[v]);
   }
+  const f32x2 rstd2 = f2_both(rstd);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    float w[8], b[8];
-    ln_param<G, VEC>(a.weight, a.param_bf16, t, v, a.cols, 1.f, w);
-    ln_param<G, VEC>(a.bias, a.param_bf16, t, v, a.cols, 0.f, b);
+    f32x2 w[4], b[4];
+    if (TABLE) {
+      ln_table_get<G>(table, t, v, w);
+      ln_table_get<G>(table + VPT * 8 * G, t, v, b);
+    } else {
+      ln_param<T, G, VEC>(a.weight, a.param_bf16, t, v, a.cols, 1.f, w);
+      ln_param<T, G, VEC>(a.bias, a.param_bf16, t, v, a.cols, 0.f, b);
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = fmaf((z[v][j] - mean) * rstd, w[j], b[j]);
+    for (int i = 0; i < 4; ++i) w[i] = f2_fma(f2_mul(f2_add(z[v][i], minus_mean), rstd2), w[i], b[i]);
     ln_put<T, G, VEC>(y, t, v, a.cols, w);
   }
+}
+
+// Persistent groups of G threads, rows ahead in the ring (long inputs).
+template <typename T, int G, int VPT, bool DROP, int VEC, int STAGES, bool TABLE>
+__global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 ? 1 : VPT <= 2 ? 3 : 2) ln_fwd_ring_kernel(const LnFwdArgs a) {
+  constexpr int kThreads = G < 256 ? 256 : G, kGroups = kThreads / G;
+  extern __shared__ __align__(16) unsigned char staged[];
+  __shared__ __align__(16) float slots[kGroups][2][64];
+  const int t = group_thread<G, kGroups>(), group = group_index<G, kGroups>();
+  using Ring = LnRing<T, G, VPT, VEC, 2, STAGES, kThreads>;
+  Ring ring;
+  ring.init(staged);
+  float* table = reinterpret_cast<float*>(staged + Ring::kBytes);
+  if (TABLE) {
+    ln_table_fill<T, G>(table, a.weight, a.param_bf16, a.cols, VPT, 1.f);
+    ln_table_fill<T, G>(table + VPT * 8 * G, a.bias, a.param_bf16, a.cols, VPT, 0.f);
+    __syncthreads();
+  }
+  Philox gen = {};
+  if (DROP) gen = Philox::load(a.rng);
+  const long long step = static_cast<long long>(gridDim.x) * kGroups;
+  const long long first = static_cast<long long>(blockIdx.x) * kGroups + group;
+  auto ahead = [&](int stage, long long row) {
+    if (row < a.rows) {
+      ring.copy(stage, 0, static_cast<const T*>(a.x) + row * a.x_stride, t, a.cols);
+      if (a.residual) ring.copy(stage, 1, static_cast<const T*>(a.residual) + row * a.residual_stride, t, a.cols);
+    }
+    ring.commit();
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) ahead(s, first + s * step);
+  int stage = 0, turn = 0;
+  for (long long row = first; row < a.rows; row += step) {
+    ring.wait();
+    f32x2 z[VPT][4], r[VPT][4];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      ring.get(stage, 0, t, v, a.cols, z[v]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[v][i] = 0;
+      if (a.residual) ring.get(stage, 1, t, v, a.cols, r[v]);
+    }
+    ahead(stage, row + STAGES * step);
+    if (++stage == STAGES) stage = 0;
+    ln_fwd_row<T, G, VPT, DROP, VEC, TABLE>(a, gen, row, t, z, r, slots[group][turn], table);
+    turn ^= 1;
+  }
+}
+
+// One row per group (inputs of few rows, where a ring would only lengthen the way; rows without 16-byte alignment).
+template <typename T, int G, int VPT, bool DROP, int VEC>
+__global__ void __launch_bounds__(G < 256 ? 256 : G) ln_fwd_kernel(const LnFwdArgs a) {
+  constexpr int kThreads = G < 256 ? 256 : G, kGroups = kThreads / G;
+  __shared__ __align__(16) float slots[kGroups][64];
+  const int t = group_thread<G, kGroups>(), group = group_index<G, kGroups>();
+  const long long row = static_cast<long long>(blockIdx.x) * kGroups + group;
+  if (row >= a.rows) return;
+  const void* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  f32x2 z[VPT][4], r[VPT][4];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) ln_get<T, G, VEC>(x, t, v, a.cols, z[v]);
+  if (a.residual) {
+    const void* res = static_cast<const T*>(a.residual) + row * a.residual_stride;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) ln_get<T, G, VEC>(res, t, v, a.cols, r[v]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[v][i] = 0;
+  }
+  Philox gen = {};
+  if (DROP) gen = Philox::load(a.rng);
+  ln_fwd_row<T, G, VPT, DROP, VEC, false>(a, gen, row, t, z, r, slots[group], nullptr);
 }
 
 // ---------------------------------------------------------------- backward
 
 // Where the parameter gradients of a thread's own columns add up over its rows: registers, or (rows so wide that they would
-// not fit beside the row) shared memory, one conflict-free column of it per thread.
+// not fit beside the row) shared memory, one conflict-free column of it per thread.  Pairs of columns.
 template <int VPT, bool SMEM, int THREADS>
 struct LnAcc {
-  float w[VPT][8], b[VPT][8];
-  __device__ __forceinline__ void init(float*) {
+  f32x2 w[VPT][4], b[VPT][4];
+  __device__ __forceinline__ void init(void*) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[v][j] = b[v][j] = 0.f;
+      for (int i = 0; i < 4; ++i) w[v][i] = b[v][i] = 0;
   }
-  __device__ __forceinline__ void add(int v, int j, float dw, float db) { w[v][j] += dw; b[v][j] += db; }
-  __device__ __forceinline__ float2 get(int v, int j) const { return make_float2(w[v][j], b[v][j]); }
+  __device__ __forceinline__ void add(int v, int i, f32x2 dy, f32x2 u) {
+    w[v][i] = f2_fma(dy, u, w[v][i]);
+    b[v][i] = f2_add(dy, b[v][i]);
+  }
+  __device__ __forceinline__ ulonglong2 get(int v, int i) const { return make_ulonglong2(w[v][i], b[v][i]); }
 };
 template <int VPT, int THREADS>
 struct LnAcc<VPT, true, THREADS> {
-  float2* own;
-  __device__ __forceinline__ void init(float* smem) {
-    own = reinterpret_cast<float2*>(smem) + threadIdx.x;
-    for (int i = 0; i < VPT * 8; ++i) own[i * THREADS] = make_float2(0.f, 0.f);
+  ulonglong2* own;
+  __device__ __forceinline__ void init(void* smem) {
+    own = static_cast<ulonglong2*>(smem) + threadIdx.x;
+    for (int i = 0; i < VPT * 4; ++i) own[i * THREADS] = make_ulonglong2(0, 0);
   }
-  __device__ __forceinline__ void add(int v, int j, float dw, float db) {
-    float2 s = own[(v * 8 + j) * THREADS];
-    s.x += dw;
-    s.y += db;
-    own[(v * 8 + j) * THREADS] = s;
+  __device__ __forceinline__ void add(int v, int i, f32x2 dy, f32x2 u) {
+    ulonglong2 s = own[(v * 4 + i) * THREADS];
+    s.x = f2_fma(dy, u, s.x);
+    s.y = f2_add(dy, s.y);
+    own[(v * 4 + i) * THREADS] = s;
   }
-  __device__ __forceinline__ float2 get(int v, int j) const { return own[(v * 8 + j) * THREADS]; }
+  __device__ __forceinline__ ulonglong2 get(int v, int i) const { return own[(v * 4 + i) * THREADS]; }
 };
 
 // Persistent groups: group g of CTA b takes the rows b * kGroups + g, + gridDim * kGroups, ...  A row is read once; its
 // gradient is written while the columns' sums stay with their thread, and leave once per CTA as a row of partial sums.
-template <typename T, int G, int VPT, bool DROP, bool VEC, bool SMEM>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) ln_bwd_kernel(const LnBwdArgs a) {
+// STAGES > 0: rows ahead in the ring (VEC only).  Beyond a row's end dy is zero, and with it all that is summed.
+template <typename T, int G, int VPT, bool DROP, int VEC, bool SMEM, int STAGES>
+__global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 || VPT > 2 ? 1 : 2) ln_bwd_kernel(const LnBwdArgs a) {
   constexpr int kThreads = G < 256 ? 256 : G, kGroups = kThreads / G;
-  extern __shared__ float dynamic[];
-  __shared__ float slots[kGroups][2][2][32];
-  const int t = threadIdx.x % G, group = threadIdx.x / G;
+  extern __shared__ __align__(16) unsigned char staged[];
+  __shared__ __align__(16) float slots[kGroups][2][32];
+  const int t = group_thread<G, kGroups>(), group = group_index<G, kGroups>();
   LnAcc<VPT, SMEM, kThreads> acc;
-  acc.init(dynamic);
+  acc.init(staged);
   Philox gen = {};
   if (DROP) gen = Philox::load(a.rng);
-  int turn = 0;
-  for (long long row = static_cast<long long>(blockIdx.x) * kGroups + group; row < a.rows;
-       row += static_cast<long long>(gridDim.x) * kGroups, turn ^= 1) {
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float g[VPT][8], u[VPT][8];
-    const void* dyp = static_cast<const T*>(a.dy) + row * a.dy_stride;
-    const void* zp = static_cast<const T*>(a.z) + row * a.z_stride;
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      ln_get<T, G, VEC>(dyp, t, v, a.cols, g[v]);
-      ln_get<T, G, VEC>(zp, t, v, a.cols, u[v]);
+  constexpr int kStages = STAGES > 0 ? STAGES : 1;
+  using Ring = LnRing<T, G, VPT, VEC, 2, kStages, kThreads>;
+  Ring ring;
+  ring.init(staged);
+  float* table = reinterpret_cast<float*>(staged + Ring::kBytes);      // with the ring only
+  if (STAGES > 0) {
+    ln_table_fill<T, G>(table, a.weight, a.param_bf16, a.cols, VPT, 1.f);
+    __syncthreads();
+  }
+  const long long step = static_cast<long long>(gridDim.x) * kGroups;
+  const long long first = static_cast<long long>(blockIdx.x) * kGroups + group;
+  auto ahead = [&](int stage, long long row) {
+    if (row < a.rows) {
+      ring.copy(stage, 0, static_cast<const T*>(a.dy) + row * a.dy_stride, t, a.cols);
+      ring.copy(stage, 1, static_cast<const T*>(a.z) + row * a.z_stride, t, a.cols);
     }
-    float s[2] = {0.f, 0.f};
+    ring.commit();
+  };
+  if (STAGES > 0) {
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-      float w[8];
-      ln_param<G, VEC>(a.weight, a.param_bf16, t, v, a.cols, 1.f, w);
+    for (int s = 0; s < kStages; ++s) ahead(s, first + s * step);
+  }
+  float mean = 0.f, rstd = 0.f;
+  if (first < a.rows) { mean = a.mean[first]; rstd = a.rstd[first]; }
+  const float per_col = 1.f / a.cols;
+  int stage = 0, turn = 0;
+  for (long long row = first; row < a.rows; row += step, turn ^= 1) {
+    f32x2 g[VPT][4], u[VPT][4];
+    if (STAGES > 0) {
+      ring.wait();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (ln_col<G, VEC>(t, v, j) >= a.cols) { u[v][j] = 0.f; continue; }
-        u[v][j] = (u[v][j] - mean) * rstd;
-        acc.add(v, j, g[v][j] * u[v][j], g[v][j]);
-        g[v][j] *= w[j];
-        s[0] += g[v][j];
-        s[1] = fmaf(g[v][j], u[v][j], s[1]);
+      for (int v = 0; v < VPT; ++v) {
+        ring.get(stage, 0, t, v, a.cols, g[v]);
+        ring.get(stage, 1, t, v, a.cols, u[v]);
+      }
+      ahead(stage, row + kStages * step);
+      if (++stage == kStages) stage = 0;
+    } else {
+      const void* dyp = static_cast<const T*>(a.dy) + row * a.dy_stride;
+      const void* zp = static_cast<const T*>(a.z) + row * a.z_stride;
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        ln_get<T, G, VEC>(dyp, t, v, a.cols, g[v]);
+        ln_get<T, G, VEC>(zp, t, v, a.cols, u[v]);
       }
     }
-    group_sum<G, 2>(s, &slots[group][turn][0][0]);
-    const float c2 = s[0] / a.cols, c1 = s[1] / a.cols;
+    const f32x2 minus_mean = f2_both(-mean), rstd2 = f2_both(rstd);
+    if (row + step < a.rows) { mean = a.mean[row + step]; rstd = a.rstd[row + step]; }      // the next row's, ahead of their use
+    f32x2 s0 = 0, s1 = 0;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      f32x2 w[4];
+      if (STAGES > 0) ln_table_get<G>(table, t, v, w);
+      else ln_param<T, G, VEC>(a.weight, a.param_bf16, t, v, a.cols, 1.f, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u[v][i] = f2_mul(f2_add(u[v][i], minus_mean), rstd2);
+        acc.add(v, i, g[v][i], u[v][i]);
+        g[v][i] = f2_mul(g[v][i], w[i]);
+        s0 = f2_add(s0, g[v][i]);
+        s1 = f2_fma(g[v][i], u[v][i], s1);
+      }
+    }
+    float a0, a1, b0, b1;
+    f2_split(s0, a0, a1);
+    f2_split(s1, b0, b1);
+    const float2 s = group_sum2<G>(a0 + a1, b0 + b1, slots[group][turn]);
+    const f32x2 minus_c2 = f2_both(-s.x * per_col), minus_c1 = f2_both(-s.y * per_col);
     void* out = static_cast<T*>(a.dresidual) + row * a.cols;
     void* dx = static_cast<T*>(a.dx) + row * a.cols;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      float d[8];
+      f32x2 d[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = (g[v][j] - c2 - u[v][j] * c1) * rstd;
+      for (int i = 0; i < 4; ++i) d[i] = f2_mul(f2_fma(u[v][i], minus_c1, f2_add(g[v][i], minus_c2)), rstd2);
       if (a.dz) {
-        float e[8];
+        f32x2 e[4];
         ln_get<T, G, VEC>(static_cast<const T*>(a.dz) + row * a.dz_stride, t, v, a.cols, e);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] += e[j];
+        for (int i = 0; i < 4; ++i) d[i] = f2_add(d[i], e[i]);
       }
       ln_put<T, G, VEC>(out, t, v, a.cols, d);
       if (DROP) {
-        const uint32_t kept = ln_kept<G, VEC>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, t, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = kept >> j & 1 ? d[j] * a.rate.scale : 0.f;
+        ln_drop<T, G, VEC, false>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, t, v, d, d);
         ln_put<T, G, VEC>(dx, t, v, a.cols, d);
       }
     }
   }
   if (!a.partials) return;
   float* part = a.partials + static_cast<long long>(blockIdx.x) * 2 * a.cols;
+  auto leave = [&](int c0, int c1, const ulonglong2& p) {
+    float lo, hi;
+    f2_split(p.x, lo, hi);
+    if (c0 < a.cols) part[c0] = lo;
+    if (c1 < a.cols) part[c1] = hi;
+    f2_split(p.y, lo, hi);
+    if (c0 < a.cols) part[a.cols + c0] = lo;
+    if (c1 < a.cols) part[a.cols + c1] = hi;
+  };
   if (kGroups == 1) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = ln_col<G, VEC>(t, v, j);
-        const float2 p = acc.get(v, j);
-        if (c < a.cols) { part[c] = p.x; part[a.cols + c] = p.y; }
-      }
+      for (int i = 0; i < 4; ++i) leave(ln_col<T, G, VEC>(t, v, 2 * i), ln_col<T, G, VEC>(t, v, 2 * i + 1), acc.get(v, i));
     return;
   }
-  // the groups of a CTA, summed in their order through shared memory: [group][slot][thread]
-  float2* all = reinterpret_cast<float2*>(dynamic);
+  // The groups of a CTA, summed in their order through shared memory: [group][pair][thread].  Nothing of the ring is under way
+  // any more (its last commits are of nothing), and the barrier is behind every thread's last read of it.
+  ulonglong2* all = reinterpret_cast<ulonglong2*>(staged);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) all[(group * 8 + j) * G + t] = acc.get(v, j);
+    for (int i = 0; i < 4; ++i) all[(group * 4 + i) * G + t] = acc.get(v, i);
     __syncthreads();
-    for (int i = threadIdx.x; i < 8 * G; i += kThreads) {
-      float2 sum = all[i];
-      for (int k = 1; k < kGroups; ++k) {
-        const float2 p = all[k * 8 * G + i];
-        sum.x += p.x;
-        sum.y += p.y;
+    for (int k = threadIdx.x; k < 4 * G; k += kThreads) {
+      ulonglong2 sum = all[k];
+      for (int o = 1; o < kGroups; ++o) {
+        const ulonglong2 p = all[o * 4 * G + k];
+        sum.x = f2_add(sum.x, p.x);
+        sum.y = f2_add(sum.y, p.y);
       }
-      const int c = ln_col<G, VEC>(i % G, v, i / G);
-      if (c < a.cols) { part[c] = sum.x; part[a.cols + c] = sum.y; }
+      leave(ln_col<T, G, VEC>(k % G, v, 2 * (k / G)), ln_col<T, G, VEC>(k % G, v, 2 * (k / G) + 1), sum);
     }
   }
 }
@@ -410,26 +658,62 @@ static bool misaligned(const void* p, uintptr_t bytes) { return reinterpret_cast
 
 static bool rows_aligned(const void* p, long long stride, uintptr_t es) { return !p || (aligned16(p) && stride * es % 16 == 0); }
 
-template <typename T, int G, int VPT, bool VEC>
-static void run_ln_fwd(const LnFwdArgs& a, cudaStream_t stream) {
-  constexpr int kThreads = G < 256 ? 256 : G, kGroups = kThreads / G;
+// The limit without the attribute counts static shared memory too.
+template <typename K>
+static int allow_smem(K kernel, uint32_t bytes) {
+  if (bytes <= 32 * 1024) return HYC_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  return e == cudaSuccess ? HYC_OK : cuda_fail(e, "cudaFuncSetAttribute");
+}
+
+// Rows ahead by what shared memory holds beside `table` bytes: two CTAs of 256 threads an SM, or one of 512.  Fewer than
+// two: no ring.
+template <typename T, int VPT, int THREADS>
+constexpr int ln_stages(int table, int most) {
+  const int stage = 2 * VPT * 8 * static_cast<int>(sizeof(T)) * THREADS, fit = ((THREADS == 512 ? 220 : 110) * 1024 - table) / stage;
+  return fit > most ? most : fit < 2 ? 0 : fit;
+}
+
+template <typename T, int G, int VPT, bool DROP, int VEC>
+static int run_ln_fwd(const LnFwdArgs& a, cudaStream_t stream) {
+  constexpr int kThreads = G < 256 ? 256 : G, kGroups = kThreads / G, kTable = 2 * VPT * 8 * G * 4;
+  constexpr bool kHasTable = kTable <= 64 * 1024;
+  constexpr int kStages = VEC ? ln_stages<T, VPT, kThreads>(kHasTable ? kTable : 0, 2) : 0;
+  if constexpr (kStages > 0) {
+    if (a.rows >= 4LL * kGroups * sm_count()) {
+      auto kernel = ln_fwd_ring_kernel<T, G, VPT, DROP, VEC, kStages, kHasTable>;
+      constexpr uint32_t smem = LnRing<T, G, VPT, VEC, 2, kStages, kThreads>::kBytes + (kHasTable ? kTable : 0);
+      const int rc = allow_smem(kernel, smem);
+      if (rc) return rc;
+      const long long batches = (a.rows + kGroups - 1) / kGroups;
+      kernel<<<resident_grid(kernel, kThreads, smem, static_cast<int>(batches < 1 << 20 ? batches : 1 << 20)), kThreads, smem, stream>>>(a);
+      return HYC_OK;
+    }
+  }
   const unsigned grid = static_cast<unsigned>((a.rows + kGroups - 1) / kGroups);
-  if (a.rng) ln_fwd_kernel<T, G, VPT, true, VEC><<<grid, kThreads, 0, stream>>>(a);
-  else ln_fwd_kernel<T, G, VPT, false, VEC><<<grid, kThreads, 0, stream>>>(a);
+  ln_fwd_kernel<T, G, VPT, DROP, VEC><<<grid, kThreads, 0, stream>>>(a);
+  return HYC_OK;
+}
+
+template <typename T, int G, int VPT>
+static int pick_ln_fwd_kind(const LnFwdArgs& a, bool vec, cudaStream_t stream) {
+  if (!vec) return a.rng ? run_ln_fwd<T, G, VPT, true, 0>(a, stream) : run_ln_fwd<T, G, VPT, false, 0>(a, stream);
+  if (a.cols != G * VPT * 8) return a.rng ? run_ln_fwd<T, G, VPT, true, 1>(a, stream) : run_ln_fwd<T, G, VPT, false, 1>(a, stream);
+  return a.rng ? run_ln_fwd<T, G, VPT, true, 2>(a, stream) : run_ln_fwd<T, G, VPT, false, 2>(a, stream);
 }
 
 // threads per row and pieces per thread by the row's width: the smallest group that holds it in at most 32 elements per thread
-template <typename T, bool VEC>
-static void pick_ln_fwd(const LnFwdArgs& a, cudaStream_t stream) {
-  const int pieces = (a.cols + 7) / 8;
-  if (pieces <= 32) run_ln_fwd<T, 32, 1, VEC>(a, stream);
-  else if (pieces <= 64) run_ln_fwd<T, 32, 2, VEC>(a, stream);
-  else if (pieces <= 96) run_ln_fwd<T, 32, 3, VEC>(a, stream);
-  else if (pieces <= 128) run_ln_fwd<T, 32, 4, VEC>(a, stream);
-  else if (pieces <= 256) run_ln_fwd<T, 128, 2, VEC>(a, stream);
-  else if (pieces <= 512) run_ln_fwd<T, 128, 4, VEC>(a, stream);
-  else if (pieces <= 1024) run_ln_fwd<T, 256, 4, VEC>(a, stream);
-  else run_ln_fwd<T, 512, 4, VEC>(a, stream);
+template <typename T>
+static int pick_ln_fwd(const LnFwdArgs& a, bool vec, cudaStream_t stream) {
+  const int slots = (a.cols + 7) / 8;
+  if (slots <= 32) return pick_ln_fwd_kind<T, 32, 1>(a, vec, stream);
+  if (slots <= 64) return pick_ln_fwd_kind<T, 32, 2>(a, vec, stream);
+  if (slots <= 96) return pick_ln_fwd_kind<T, 32, 3>(a, vec, stream);
+  if (slots <= 128) return pick_ln_fwd_kind<T, 32, 4>(a, vec, stream);
+  if (slots <= 256) return pick_ln_fwd_kind<T, 128, 2>(a, vec, stream);
+  if (slots <= 512) return pick_ln_fwd_kind<T, 256, 2>(a, vec, stream);
+  if (slots <= 1024) return pick_ln_fwd_kind<T, 512, 2>(a, vec, stream);
+  return pick_ln_fwd_kind<T, 512, 4>(a, vec, stream);
 }
 
 template <typename T>
@@ -437,19 +721,22 @@ static int launch_ln_fwd(const LnFwdArgs& a, cudaStream_t stream) {
   const uintptr_t es = sizeof(T);
   const bool vec = a.cols % 8 == 0 && rows_aligned(a.x, a.x_stride, es) && rows_aligned(a.residual, a.residual_stride, es) &&
                    aligned16(a.y) && aligned16(a.z) && aligned16(a.weight) && aligned16(a.bias);
-  if (vec) pick_ln_fwd<T, true>(a, stream);
-  else pick_ln_fwd<T, false>(a, stream);
+  const int rc = pick_ln_fwd<T>(a, vec, stream);
+  if (rc) return rc;
   HYC_LAUNCHED();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? HYC_OK : cuda_fail(e, "ln_fwd_kernel");
 }
 
-template <typename T, int G, int VPT, bool DROP, bool VEC, bool SMEM>
+template <typename T, int G, int VPT, bool DROP, int VEC, bool SMEM>
 static int run_ln_bwd(LnBwdArgs a, cudaStream_t stream) {
   constexpr int kThreads = G < 256 ? 256 : G, kGroups = kThreads / G;
-  auto kernel = ln_bwd_kernel<T, G, VPT, DROP, VEC, SMEM>;
-  const uint32_t smem = SMEM ? kThreads * VPT * 8 * 8 : kGroups > 1 ? kThreads * 8 * 8 : 0;
-  const int rc = set_smem(kernel, smem);
+  constexpr int kTable = VPT * 8 * G * 4, kStages = VEC && !SMEM ? ln_stages<T, VPT, kThreads>(kTable, 2) : 0;
+  auto kernel = ln_bwd_kernel<T, G, VPT, DROP, VEC, SMEM, kStages>;
+  constexpr uint32_t sums = SMEM ? kThreads * VPT * 8 * 8 : kGroups > 1 ? kThreads * 8 * 8 : 0;
+  constexpr uint32_t ahead = kStages ? LnRing<T, G, VPT, VEC, 2, kStages ? kStages : 1, kThreads>::kBytes + kTable : 0;
+  constexpr uint32_t smem = sums > ahead ? sums : ahead;
+  const int rc = allow_smem(kernel, smem);
   if (rc) return rc;
   const long long batches = (a.rows + kGroups - 1) / kGroups;
   a.parts = resident_grid(kernel, kThreads, smem, static_cast<int>(batches < kLnMaxParts ? batches : kLnMaxParts));
@@ -463,17 +750,24 @@ static int run_ln_bwd(LnBwdArgs a, cudaStream_t stream) {
   return e == cudaSuccess ? HYC_OK : cuda_fail(e, "ln_bwd_kernel");
 }
 
-template <typename T, bool DROP, bool VEC>
-static int pick_ln_bwd(const LnBwdArgs& a, cudaStream_t stream) {
-  const int pieces = (a.cols + 7) / 8;
-  if (pieces <= 32) return run_ln_bwd<T, 32, 1, DROP, VEC, false>(a, stream);
-  if (pieces <= 64) return run_ln_bwd<T, 32, 2, DROP, VEC, false>(a, stream);
-  if (pieces <= 96) return run_ln_bwd<T, 32, 3, DROP, VEC, false>(a, stream);
-  if (pieces <= 128) return run_ln_bwd<T, 128, 1, DROP, VEC, false>(a, stream);
-  if (pieces <= 256) return run_ln_bwd<T, 128, 2, DROP, VEC, false>(a, stream);
-  if (pieces <= 512) return run_ln_bwd<T, 256, 2, DROP, VEC, false>(a, stream);
-  if (pieces <= 1024) return run_ln_bwd<T, 512, 2, DROP, VEC, false>(a, stream);
-  return run_ln_bwd<T, 512, 4, DROP, VEC, true>(a, stream);
+template <typename T, int G, int VPT, bool SMEM>
+static int pick_ln_bwd_kind(const LnBwdArgs& a, bool vec, cudaStream_t stream) {
+  if (!vec) return a.rng ? run_ln_bwd<T, G, VPT, true, 0, SMEM>(a, stream) : run_ln_bwd<T, G, VPT, false, 0, SMEM>(a, stream);
+  if (a.cols != G * VPT * 8) return a.rng ? run_ln_bwd<T, G, VPT, true, 1, SMEM>(a, stream) : run_ln_bwd<T, G, VPT, false, 1, SMEM>(a, stream);
+  return a.rng ? run_ln_bwd<T, G, VPT, true, 2, SMEM>(a, stream) : run_ln_bwd<T, G, VPT, false, 2, SMEM>(a, stream);
+}
+
+template <typename T>
+static int pick_ln_bwd(const LnBwdArgs& a, bool vec, cudaStream_t stream) {
+  const int slots = (a.cols + 7) / 8;
+  if (slots <= 32) return pick_ln_bwd_kind<T, 32, 1, false>(a, vec, stream);
+  if (slots <= 64) return pick_ln_bwd_kind<T, 32, 2, false>(a, vec, stream);
+  if (slots <= 96) return pick_ln_bwd_kind<T, 32, 3, false>(a, vec, stream);
+  if (slots <= 128) return pick_ln_bwd_kind<T, 128, 1, false>(a, vec, stream);
+  if (slots <= 256) return pick_ln_bwd_kind<T, 128, 2, false>(a, vec, stream);
+  if (slots <= 512) return pick_ln_bwd_kind<T, 256, 2, false>(a, vec, stream);
+  if (slots <= 1024) return pick_ln_bwd_kind<T, 512, 2, false>(a, vec, stream);
+  return pick_ln_bwd_kind<T, 512, 4, true>(a, vec, stream);
 }
 
 template <typename T>
@@ -481,8 +775,7 @@ static int launch_ln_bwd(const LnBwdArgs& a, cudaStream_t stream) {
   const uintptr_t es = sizeof(T);
   const bool vec = a.cols % 8 == 0 && rows_aligned(a.dy, a.dy_stride, es) && rows_aligned(a.z, a.z_stride, es) &&
                    rows_aligned(a.dz, a.dz_stride, es) && aligned16(a.dresidual) && aligned16(a.dx) && aligned16(a.weight);
-  if (vec) return a.rng ? pick_ln_bwd<T, true, true>(a, stream) : pick_ln_bwd<T, false, true>(a, stream);
-  return a.rng ? pick_ln_bwd<T, true, false>(a, stream) : pick_ln_bwd<T, false, false>(a, stream);
+  return pick_ln_bwd<T>(a, vec, stream);
 }
 
 }  // namespace hyc
