@@ -163,7 +163,9 @@ template <typename T, bool RES, int U>
 static void run_dropout_flat(const DropoutArgs& a, cudaStream_t stream) {
   auto kernel = dropout_flat_kernel<T, RES, U>;
   const long long blocks = a.cols / (256 * U * (16 / sizeof(T))) + 1;
-  kernel<<<resident_grid(kernel, 256, 0, static_cast<int>(blocks < 1 << 20 ? blocks : 1 << 20)), 256, 0, stream>>>(a);
+  static PerDevice resident;
+  const long long most = resident.get([&] { return resident_grid(kernel, 256, 0, 1 << 20); });
+  kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(a);
 }
 
 template <typename T>

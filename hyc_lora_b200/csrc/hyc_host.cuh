@@ -146,6 +146,22 @@ inline int resident_grid(K kernel, int threads, uint32_t smem_bytes, int grid) {
   return grid > cap ? static_cast<int>(cap) : grid;
 }
 
+// A positive number worked out once per device (what an occupancy query answers, an attribute that has been set).
+struct PerDevice {
+  std::atomic<int> value[64];
+  template <typename F>
+  int get(F make) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return make();
+    int v = value[dev].load(std::memory_order_relaxed);
+    if (v == 0) {
+      v = make();
+      value[dev].store(v, std::memory_order_relaxed);
+    }
+    return v;
+  }
+};
+
 template <typename K>
 inline int set_smem(K kernel, uint32_t bytes) {
   if (bytes <= 48 * 1024) return HYC_OK;

@@ -658,12 +658,14 @@ static bool misaligned(const void* p, uintptr_t bytes) { return reinterpret_cast
 
 static bool rows_aligned(const void* p, long long stride, uintptr_t es) { return !p || (aligned16(p) && stride * es % 16 == 0); }
 
-// The limit without the attribute counts static shared memory too.
+// CTAs of a kernel that the device holds at once, with the shared memory it asks for allowed first (without the attribute the
+// limit counts static shared memory too); 0: refused.  Worked out once per device and kernel.
 template <typename K>
-static int allow_smem(K kernel, uint32_t bytes) {
-  if (bytes <= 32 * 1024) return HYC_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-  return e == cudaSuccess ? HYC_OK : cuda_fail(e, "cudaFuncSetAttribute");
+static int ln_resident(PerDevice& cache, K kernel, int threads, uint32_t smem) {
+  return cache.get([&] {
+    if (smem > 32 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return 0;
+    return resident_grid(kernel, threads, smem, 1 << 20);
+  });
 }
 
 // Rows ahead by what shared memory holds beside `table` bytes: two CTAs of 256 threads an SM, or one of 512.  Fewer than
@@ -683,10 +685,10 @@ static int run_ln_fwd(const LnFwdArgs& a, cudaStream_t stream) {
     if (a.rows >= 4LL * kGroups * sm_count()) {
       auto kernel = ln_fwd_ring_kernel<T, G, VPT, DROP, VEC, kStages, kHasTable>;
       constexpr uint32_t smem = LnRing<T, G, VPT, VEC, 2, kStages, kThreads>::kBytes + (kHasTable ? kTable : 0);
-      const int rc = allow_smem(kernel, smem);
-      if (rc) return rc;
-      const long long batches = (a.rows + kGroups - 1) / kGroups;
-      kernel<<<resident_grid(kernel, kThreads, smem, static_cast<int>(batches < 1 << 20 ? batches : 1 << 20)), kThreads, smem, stream>>>(a);
+      static PerDevice resident;
+      const long long most = ln_resident(resident, kernel, kThreads, smem), batches = (a.rows + kGroups - 1) / kGroups;
+      if (most < 1) return cuda_fail(cudaGetLastError(), "cudaFuncSetAttribute");
+      kernel<<<static_cast<unsigned>(batches < most ? batches : most), kThreads, smem, stream>>>(a);
       return HYC_OK;
     }
   }
@@ -736,10 +738,11 @@ static int run_ln_bwd(LnBwdArgs a, cudaStream_t stream) {
   constexpr uint32_t sums = SMEM ? kThreads * VPT * 8 * 8 : kGroups > 1 ? kThreads * 8 * 8 : 0;
   constexpr uint32_t ahead = kStages ? LnRing<T, G, VPT, VEC, 2, kStages ? kStages : 1, kThreads>::kBytes + kTable : 0;
   constexpr uint32_t smem = sums > ahead ? sums : ahead;
-  const int rc = allow_smem(kernel, smem);
-  if (rc) return rc;
-  const long long batches = (a.rows + kGroups - 1) / kGroups;
-  a.parts = resident_grid(kernel, kThreads, smem, static_cast<int>(batches < kLnMaxParts ? batches : kLnMaxParts));
+  static PerDevice resident;
+  const long long most = ln_resident(resident, kernel, kThreads, smem), batches = (a.rows + kGroups - 1) / kGroups;
+  if (most < 1) return cuda_fail(cudaGetLastError(), "cudaFuncSetAttribute");
+  a.parts = static_cast<int>(batches < most ? batches : most);
+  if (a.parts > kLnMaxParts) a.parts = kLnMaxParts;
   kernel<<<a.parts, kThreads, smem, stream>>>(a);
   HYC_LAUNCHED();
   if (a.partials) {
