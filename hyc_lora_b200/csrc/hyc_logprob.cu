@@ -10,12 +10,16 @@
 
 #include "hyc_host.cuh"
 
+#ifndef LPM
+#define LPM 512
+#define LPA 4
+#endif
 namespace hyc {
 
 struct LogprobArgs {
   const void* logits;
-  long long rows, row_stride, batch_stride, seq;
-  int vocab, top;
+  long long row_stride, batch_stride;
+  int rows, seq, vocab, top;               // seq >= rows: one stride
   const long long* targets;
   long long ignore_index;
   float *logprob, *entropy, *stats, *top_logprob;
@@ -24,8 +28,8 @@ struct LogprobArgs {
 
 struct LogprobBwdArgs {
   const void* logits;
-  long long rows, row_stride, batch_stride, seq;
-  int vocab, top;
+  long long row_stride, batch_stride;
+  int rows, seq, vocab, top;
   const long long* targets;
   long long ignore_index;
   const float *stats, *entropy, *d_logprob, *d_entropy, *d_top;
@@ -56,9 +60,9 @@ __device__ __forceinline__ float lp_max(float a, float b) {
   return r;
 }
 __device__ __forceinline__ float lp_warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = lp_max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 // 2^x to about 2^-22, results below the normal numbers as zero
 __device__ __forceinline__ float lp_exp2(float x) {
@@ -70,22 +74,35 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ---------------------------------------------------------------- forward
 
-// A row (or, in a cluster, a CTA's slice of one) is held in registers, kPer 16-byte pieces per thread, and read once.
-//   1. its largest value (packed maxima), over the CTA;
-//   2. the sums of e = exp(x - m) and e (x - m), with what equals m counted apart -- only the warps that hold it test for it;
-//      each piece's register takes the next row's piece as soon as it is spent, so that loads run through the reductions;
-//   3. alternatives: the k-th largest of 64 groups' maxima is a bound that the k best reach and hardly anything else does.
-//      The few values that reach it are collected, and each counts those before it.  Where too many reach it (rows of equal
-//      values, or hardly anything open), or the row holds a NaN, the best are picked one after the other instead.
-// The CTAs of a cluster work on slices with their own m; the first one joins sums and alternatives through distributed shared
-// memory, in rank order: no atomics on results, no workspace, one launch.
-constexpr int kLpCandidates = 256, kLpGroups = 64;
+// Persistent CTAs, a row at a time; a row is streamed once, in chunks of kLpChunk 16-byte pieces per thread, the next chunk (of
+// this row or the next) in flight while one is worked on.  Within a row the warps go their own ways:
+//   1. a warp keeps a largest value m of what it has seen, and the sums of e = exp(x - m) and e (x - m), with what equals m
+//      counted apart.  A chunk whose own largest is below m is summed as it stands; else the sums so far are scaled to the new
+//      m, and the values of the pieces that hold it are tested for it.  At the row's end the warps' sums are joined.
+//   2. alternatives: every thread also knows the largest value it has seen.  The k-th largest of 64 groups' maxima is a bound
+//      that the k best reach and hardly anything else does; the few threads that have seen something that reaches it have
+//      their pieces read again (from L2) by the whole CTA, what reaches the bound is collected, and each counts those before
+//      it.  Where too many reach it (rows of equal values, or hardly anything open), or the row holds a NaN, the best are
+//      picked one after the other instead.
+// Few long rows are split over the CTAs of a cluster, which work on slices with their own m; the first one joins sums and
+// alternatives through distributed shared memory, in rank order: no atomics on results, no workspace, one launch.
+//
+// Issue slots are as scarce as bytes here: bf16 leaves 11 of them per 32 elements at full bandwidth, and the exponentials take
+// 8 of their unit's cycles.  Holding whole rows in registers instead, with a barrier behind the maximum and one behind the
+// sums, took 122 us at 8192 x 32000 (512 threads of 8 pieces) or 186 (256 of 16); staging them in shared memory 151.
+constexpr int kLpCandidates = 256, kLpGroups = 64, kLpChunk = 4;
 
-__host__ __device__ constexpr int lp_per(int threads) { return threads > 512 ? 16 : 8; }
-
-struct LpSums {
+struct alignas(16) LpSums {        // stored by 16 bytes into another CTA's shared memory
   float m, count, rest, te;     // largest, how often, sum of the other e, sum of e (x - m)
 };
+
+// elements between the first row's start and this one's
+template <typename A>
+__device__ __forceinline__ long long lp_offset(const A& a, int row) {
+  if (a.seq >= a.rows) return row * a.row_stride;
+  const unsigned batch = static_cast<unsigned>(row) / static_cast<unsigned>(a.seq);
+  return batch * a.batch_stride + (row - static_cast<int>(batch) * a.seq) * a.row_stride;
+}
 
 template <typename T>
 __device__ __forceinline__ float lp_piece_max(const uint4& w);
@@ -114,34 +131,40 @@ __device__ __forceinline__ void lp_unpack<float>(const uint4& w, float (&f)[4]) 
 struct LpRow {
   const unsigned char* base;   // 16-byte aligned
   int lead;                    // elements of the first piece that belong to what is before the row
-  int first, pieces;           // this CTA's pieces
+  int first, pieces;           // this CTA's pieces; may be <= 0
+  int from, whole;             // of those, [from, from + whole) lie wholly inside the row
 };
 
 template <typename T>
 __device__ __forceinline__ LpRow lp_row(const void* logits, long long offset, int vocab, int rank, int ranks) {
+  constexpr int kPiece = 16 / sizeof(T);
   const unsigned char* p = static_cast<const unsigned char*>(logits) + offset * static_cast<long long>(sizeof(T));
   LpRow r;
   const int phase = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u);
   r.base = p - phase;
   r.lead = phase / static_cast<int>(sizeof(T));
-  const int all = (r.lead + vocab + 16 / static_cast<int>(sizeof(T)) - 1) / (16 / static_cast<int>(sizeof(T)));
-  const int each = (all + ranks - 1) / ranks;
-  r.first = rank * each;
-  r.pieces = min(each, all - r.first);      // may be <= 0
+  const int all = (r.lead + vocab + kPiece - 1) / kPiece;
+  r.first = 0;
+  r.pieces = all;
+  if (ranks > 1) {
+    const int each = (all + ranks - 1) / ranks;
+    r.first = rank * each;
+    r.pieces = min(each, all - r.first);
+  }
+  const int begin = r.lead ? 1 : 0, end = (r.lead + vocab) / kPiece;
+  r.from = max(begin - r.first, 0);
+  r.whole = max(min(end - r.first, r.pieces) - r.from, 0);
   return r;
 }
 
-// piece `i` of the slice; what lies outside the row is not read and counts as -inf
+// piece `i` of the slice, a ragged end of the row: element by element, shifted in from above; -inf outside the row
 template <typename T>
-__device__ __forceinline__ uint4 lp_fetch(const LpRow& r, int vocab, int i) {
+__device__ __forceinline__ uint4 lp_ragged(const LpRow& r, int vocab, int i) {
   constexpr int kPiece = 16 / sizeof(T);
   const uint32_t shut = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
   uint4 w = make_uint4(shut, shut, shut, shut);
-  if (i >= r.pieces) return w;
   const int piece = r.first + i, e0 = piece * kPiece - r.lead;
   const unsigned char* p = r.base + static_cast<long long>(piece) * 16;
-  if (e0 >= 0 && e0 + kPiece <= vocab) return load16_stream(p);
-  // a row's ragged end: element by element, shifted in from above
 #pragma unroll 1
   for (int e = 0; e < kPiece; ++e) {
     const bool in = e0 + e >= 0 && e0 + e < vocab;
@@ -159,13 +182,52 @@ __device__ __forceinline__ uint4 lp_fetch(const LpRow& r, int vocab, int i) {
   return w;
 }
 
-// sums of one piece; APART: values equal to m are counted instead
+// piece `i` of the slice; what lies outside the row is not read and counts as -inf
+template <typename T>
+__device__ __forceinline__ uint4 lp_fetch(const LpRow& r, int vocab, int i) {
+  if (static_cast<unsigned>(i - r.from) < static_cast<unsigned>(r.whole))
+    return load16_stream(r.base + static_cast<long long>(r.first + i) * 16);
+  if (i < r.pieces && i >= 0) return lp_ragged<T>(r, vocab, i);
+  const uint32_t shut = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+  return make_uint4(shut, shut, shut, shut);
+}
+
+// A thread's pieces t, t + THREADS, ...: chunk k is those of the sweeps 4 k .. 4 k + 3.  Chunks of whole pieces cost their
+// loads and a uniform branch.
+template <typename T, int THREADS>
+struct LpSweep {
+  LpRow r;
+  const unsigned char* own;    // the thread's piece of sweep 0
+  int begin, plain;            // chunks [begin, plain) are whole
+  int chunks;
+  __device__ __forceinline__ void start(const void* logits, long long offset, int vocab, int rank, int ranks) {
+    r = lp_row<T>(logits, offset, vocab, rank, ranks);
+    own = r.base + (static_cast<long long>(r.first) + threadIdx.x) * 16;
+    begin = r.from > 0 ? 1 : 0;
+    plain = (r.from + r.whole) / (THREADS * kLpChunk);
+    chunks = r.pieces > 0 ? (r.pieces + THREADS * kLpChunk - 1) / (THREADS * kLpChunk) : 0;
+  }
+  __device__ __forceinline__ void load(int k, int vocab, uint4 (&w)[kLpChunk]) const {
+    if (k >= begin && k < plain) {
+      const unsigned char* p = own + static_cast<long long>(k) * (THREADS * kLpChunk * 16);
+#pragma unroll
+      for (int i = 0; i < kLpChunk; ++i) w[i] = load16_stream(p + i * (THREADS * 16));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLpChunk; ++i) w[i] = lp_fetch<T>(r, vocab, (k * kLpChunk + i) * THREADS + static_cast<int>(threadIdx.x));
+    }
+  }
+};
+
+// Sums of one piece in base 2: with L = log2 e in fp32 and c = -m L rounded, u = x L + c in one rounding, e = 2^u; what c lost
+// to its rounding is a common factor that the row's sums are given at the end (lp_rescale).  APART: values equal to m are
+// counted instead.
 template <typename T, bool ENT, bool APART>
-__device__ __forceinline__ void lp_piece_sums(const uint4& w, float m, f32x2& rest, f32x2& te, float& count) {
+__device__ __forceinline__ void lp_piece_sums(const uint4& w, float m, f32x2 c, f32x2& rest, f32x2& te, float& count) {
   constexpr int kPiece = 16 / sizeof(T);
   float f[kPiece];
   lp_unpack<T>(w, f);
-  const f32x2 minus_m = f2_make(-m, -m), log2e = f2_make(kLog2e, kLog2e);
+  const f32x2 log2e = f2_make(kLog2e, kLog2e);
 #pragma unroll
   for (int i = 0; i < kPiece / 2; ++i) {
     float x0 = f[2 * i], x1 = f[2 * i + 1];
@@ -173,19 +235,27 @@ __device__ __forceinline__ void lp_piece_sums(const uint4& w, float m, f32x2& re
       if (x0 == m) { count += 1.f; x0 = -INFINITY; }
       if (x1 == m) { count += 1.f; x1 = -INFINITY; }
     }
-    f32x2 d = f2_add(f2_make(x0, x1), minus_m);
-    if (ENT) {
-      // e is 0 long before; a finite difference keeps 0 * d at 0 (and max.NaN keeps a NaN)
-      float d0, d1;
-      f2_split(d, d0, d1);
-      d = f2_make(lp_max(d0, -10000.f), lp_max(d1, -10000.f));
-    }
+    f32x2 u = f2_fma(f2_make(x0, x1), log2e, c);
     float u0, u1;
-    f2_split(f2_mul(d, log2e), u0, u1);
+    f2_split(u, u0, u1);
+    if (ENT) {
+      // e is 0 long before; a finite u keeps 0 * u at 0 (and max.NaN keeps a NaN)
+      u0 = lp_max(u0, -10000.f);
+      u1 = lp_max(u1, -10000.f);
+      u = f2_make(u0, u1);
+    }
     const f32x2 e = f2_make(lp_exp2(u0), lp_exp2(u1));
     rest = f2_add(rest, e);
-    if (ENT) te = f2_fma(e, d, te);
+    if (ENT) te = f2_fma(e, u, te);
   }
+}
+
+// sum of e and of e u -> sum of e and of e (x - m)
+__device__ __forceinline__ void lp_rescale(float m, float c, float& rest, float& te) {
+  const float lost = fmaf(-m, kLog2e, -c);             // exact
+  const float factor = exp2f(lost);
+  te = (te + lost * rest) * factor * 0.6931471805599453f;
+  rest *= factor;
 }
 
 // the best `top` of this CTA's slice one after the other, from memory (rare: see above); keys in descending order to `out`
@@ -222,47 +292,50 @@ __device__ __noinline__ void lp_pick_slowly(const LpRow r, int vocab, int top, u
   __syncthreads();
 }
 
-template <int THREADS>
 struct LpShared {
-  float4 wmax4[2][8];                      // [parity][warps], as float
-  LpSums part[2][32];                      // [parity][warp]
-  float group[kLpGroups];
+  LpSums part[2][8];                       // [parity][warp]
+  float4 group[kLpGroups / 4];
   float bound;
-  int found;
+  int hot, found;
+  unsigned short hots[256];                // threads that have seen something that reaches the bound
   unsigned long long keys[kLpCandidates];
   unsigned long long picked[32];
-  unsigned long long best[32];
-  float2 result;                           // m, log S of the row (one CTA per row)
+  unsigned long long best[8];
+  float2 result;                           // m, log S of the row
   LpSums slice[2][8];                      // [parity][rank], in the first CTA of a cluster
   unsigned long long slice_keys[2][8][32];
 };
 
-__device__ __forceinline__ LpSums lp_join(const LpSums* s, int n) {
-  float m = s[0].m;
-  for (int i = 1; i < n; ++i) m = lp_max(m, s[i].m);
+// sums of up to eight parts, one per lane; complete in the first eight lanes
+__device__ __forceinline__ LpSums lp_join(LpSums s, bool have) {
+  if (!have) s.m = -INFINITY;
+  const float m = lp_warp_max(s.m);
   LpSums r = {m, 0.f, 0.f, 0.f};
-  for (int i = 0; i < n; ++i) {
-    if (s[i].m == -INFINITY) continue;     // nothing open there
-    if (s[i].m == m) {
-      r.count += s[i].count;
-      r.rest += s[i].rest;
-      r.te += s[i].te;
-    } else {
-      const float d = s[i].m - m, f = expf(d), sum = s[i].count + s[i].rest;
-      r.rest += sum * f;
-      r.te += f == 0.f ? 0.f : f * (s[i].te + d * sum);
-    }
+  if (s.m == -INFINITY) {
+    // nothing open there
+  } else if (s.m == m) {
+    r = s;
+  } else {
+    const float d = s.m - m, f = expf(d), sum = s.count + s.rest;
+    r.rest = sum * f;
+    r.te = f == 0.f ? 0.f : f * (s.te + d * sum);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    r.count += __shfl_xor_sync(0xffffffffu, r.count, o);
+    r.rest += __shfl_xor_sync(0xffffffffu, r.rest, o);
+    r.te += __shfl_xor_sync(0xffffffffu, r.te, o);
   }
   return r;
 }
 
 // one thread: the row's results from its sums; returns (m, log S) with log S NaN where the row has a NaN or +inf
-__device__ __forceinline__ float2 lp_finish(const LogprobArgs& a, long long row, const LpSums& s, long long target, float at_target) {
+__device__ __forceinline__ float2 lp_finish(const LogprobArgs& a, int row, const LpSums& s, long long target, float at_target) {
   const bool none = s.m == -INFINITY;
   float logz = s.count == 1.f ? log1pf(s.rest) : logf(s.count + s.rest);
   if (none) logz = 0.f;
   if (!(s.m < INFINITY)) logz = NAN;
-  *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(s.m, logz);
+  *reinterpret_cast<float2*>(a.stats + 2LL * row) = make_float2(s.m, logz);
   if (a.entropy) a.entropy[row] = none ? 0.f : logz - s.te / (s.count + s.rest);
   if (a.targets) {
     float lp = NAN;                                                  // a target outside the vocabulary
@@ -273,9 +346,9 @@ __device__ __forceinline__ float2 lp_finish(const LogprobArgs& a, long long row,
   return make_float2(s.m, logz);
 }
 
-__device__ __forceinline__ void lp_put_top(const LogprobArgs& a, long long row, int rank, unsigned long long key, float2 mz) {
-  a.top_index[row * a.top + rank] = lp_key_index(key);
-  a.top_logprob[row * a.top + rank] = mz.x == -INFINITY ? -INFINITY : lp_key_value(key) - mz.x - mz.y;
+__device__ __forceinline__ void lp_put_top(const LogprobArgs& a, int row, int rank, unsigned long long key, float2 mz) {
+  a.top_index[static_cast<long long>(row) * a.top + rank] = lp_key_index(key);
+  a.top_logprob[static_cast<long long>(row) * a.top + rank] = mz.x == -INFINITY ? -INFINITY : lp_key_value(key) - mz.x - mz.y;
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -298,108 +371,68 @@ __device__ __forceinline__ uint32_t in_first_cta(const void* p) {
   return r;
 }
 
-template <typename T, int THREADS, bool ENT, bool TOP, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, THREADS > 512 ? 1 : 1024 / THREADS) logprob_kernel(const LogprobArgs a) {
-  constexpr int kPiece = 16 / sizeof(T), kPer = lp_per(THREADS), kWarps = THREADS / 32;
-  constexpr int kPerGroup = THREADS <= kLpGroups ? 1 : THREADS > 512 ? 16 : THREADS / kLpGroups;   // lanes of a group, a power of two
-  __shared__ LpShared<THREADS> sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0, ranks = CLUSTER ? static_cast<int>(cluster_size()) : 1;
-  const long long step = gridDim.x / ranks;
-  if (TOP && threadIdx.x == 0) sh.found = 0;
-  auto at = [&](long long row) {
-    const long long batch = row / a.seq;
-    return batch * a.batch_stride + (row - batch * a.seq) * a.row_stride;
-  };
-  // rows without a target of which nothing else is asked are not read
-  auto next = [&](long long row) {
-    if (!ENT && !TOP && a.targets) {
-      while (row < a.rows && a.targets[row] == a.ignore_index) {
-        if (rank == 0 && threadIdx.x == 0) {
-          a.logprob[row] = 0.f;
-          *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(-INFINITY, 0.f);
-        }
-        row += step;
-      }
-    }
-    return row;
-  };
-  uint4 raw[kPer];
-  long long row = next(blockIdx.x / ranks);
-  LpRow r = {};
-  long long target = -1;
-  float at_target = 0.f;
-  auto head = [&](long long to) {            // what the first thread needs of a row, beside its pieces
-    if (a.targets && rank == 0 && threadIdx.x == 0) {
-      target = a.targets[to];
-      if (target >= 0 && target < a.vocab) at_target = lp_load(static_cast<const T*>(a.logits), at(to) + target);
-    }
-  };
-  if (row < a.rows) {
-    r = lp_row<T>(a.logits, at(row), a.vocab, rank, ranks);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) raw[i] = lp_fetch<T>(r, a.vocab, i * THREADS + threadIdx.x);
-    head(row);
+// a warp's running sums (per lane) over the chunks of a row
+template <typename T, bool ENT>
+struct LpRunning {
+  float m, c, count;             // m and c = -m log2(e) of the warp
+  f32x2 rest, te;
+  bool far;                      // |m| so large that its neighbours in fp32 are 10^22 apart: e is 0 for all but m (and c may overflow)
+
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    c = count = 0.f;
+    rest = te = 0;
+    far = true;
   }
-  int turn = 0;
-  while (row < a.rows) {
-    // 1. the largest
-    float mine = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) mine = lp_max(mine, lp_piece_max<T>(raw[i]));
-    float wmax = mine;
-    if (TOP && kPerGroup <= 16) {
-#pragma unroll
-      for (int o = 1; o < kPerGroup; o <<= 1) wmax = lp_max(wmax, __shfl_xor_sync(0xffffffffu, wmax, o));
-      if (threadIdx.x % kPerGroup == 0 && threadIdx.x / kPerGroup < kLpGroups) sh.group[threadIdx.x / kPerGroup] = wmax;
-#pragma unroll
-      for (int o = kPerGroup; o < 32; o <<= 1) wmax = lp_max(wmax, __shfl_xor_sync(0xffffffffu, wmax, o));
-    } else {
-      wmax = lp_warp_max(wmax);
-    }
-    float m = wmax;
-    float* all = reinterpret_cast<float*>(sh.wmax4[turn]);
-    if (kWarps > 1 || TOP) {
-      if (lane == 0) all[warp] = wmax;
-      __syncthreads();
-      if (kWarps > 1) m = lp_warp_max(lane < kWarps ? all[lane] : -INFINITY);
-    }
-    // the bound of the alternatives, by the first warps
-    constexpr int kGroups = THREADS / kPerGroup < kLpGroups ? THREADS / kPerGroup : kLpGroups;
-    if (TOP && threadIdx.x < kGroups) {
-      const float v = sh.group[threadIdx.x];
-      int before = 0;
-#pragma unroll 8
-      for (int j = 0; j < kGroups; ++j) {
-        const float o = sh.group[j];
-        before += o > v || (o == v && j < static_cast<int>(threadIdx.x));
+  // a chunk, the thread's largest value of each piece and the warp's of all
+  __device__ __forceinline__ void add(const uint4 (&w)[kLpChunk], const float (&most)[kLpChunk], float largest) {
+    if (!(largest < m)) {
+      if (largest != m) {        // what there is, to the new m
+        const bool was_far = far;
+        const float old = c;
+        m = lp_max(m, largest);
+        far = fabsf(m) >= 1e30f;
+        c = far ? 0.f : -m * kLog2e;
+        if (was_far || far) {
+          rest = te = 0;
+        } else {
+          float lo, hi;
+          const float up = c - old, f = lp_exp2(up);
+          f2_split(rest, lo, hi);
+          const f32x2 all = f2_make(lo + count, hi), f2 = f2_make(f, f);
+          if (ENT) te = f2_mul(f2, f2_fma(f2_make(up, up), all, te));
+          rest = f2_mul(f2, all);
+        }
+        count = 0.f;
       }
-      if (before == a.top - 1) sh.bound = v;
-    }
-    // 2. the sums
-    const float base = m == -INFINITY ? 0.f : m;
-    f32x2 rest2 = 0, te2 = 0;
-    LpSums s = {m, 0.f, 0.f, 0.f};
-    const long long upcoming = next(row + step);
-    const LpRow now = r;
-    if (upcoming < a.rows) r = lp_row<T>(a.logits, at(upcoming), a.vocab, rank, ranks);
-    if (wmax == m) {
+      const f32x2 c2 = f2_make(c, c);
+      if (far) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        lp_piece_sums<T, ENT, true>(raw[i], base, rest2, te2, s.count);
-        if (!TOP && upcoming < a.rows) raw[i] = lp_fetch<T>(r, a.vocab, i * THREADS + threadIdx.x);
-      }
-    } else {
+        for (int i = 0; i < kLpChunk; ++i) {
+          float f[16 / sizeof(T)];
+          lp_unpack<T>(w[i], f);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        lp_piece_sums<T, ENT, false>(raw[i], base, rest2, te2, s.count);
-        if (!TOP && upcoming < a.rows) raw[i] = lp_fetch<T>(r, a.vocab, i * THREADS + threadIdx.x);
+          for (int e = 0; e < static_cast<int>(16 / sizeof(T)); ++e) count += f[e] == m && m != -INFINITY ? 1.f : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kLpChunk; ++i) {
+          if (__any_sync(0xffffffffu, !(most[i] < m))) lp_piece_sums<T, ENT, true>(w[i], m, c2, rest, te, count);
+          else lp_piece_sums<T, ENT, false>(w[i], m, c2, rest, te, count);
+        }
       }
+    } else if (!far) {
+      const f32x2 c2 = f2_make(c, c);
+#pragma unroll
+      for (int i = 0; i < kLpChunk; ++i) lp_piece_sums<T, ENT, false>(w[i], m, c2, rest, te, count);
     }
+  }
+  __device__ __forceinline__ LpSums warp_sums() const {
     float lo, hi;
-    f2_split(rest2, lo, hi);
+    LpSums s = {m, count, 0.f, 0.f};
+    f2_split(rest, lo, hi);
     s.rest = lo + hi;
-    f2_split(te2, lo, hi);
+    f2_split(te, lo, hi);
     s.te = lo + hi;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -407,84 +440,178 @@ __global__ void __launch_bounds__(THREADS, THREADS > 512 ? 1 : 1024 / THREADS) l
       s.rest += __shfl_xor_sync(0xffffffffu, s.rest, o);
       if (ENT) s.te += __shfl_xor_sync(0xffffffffu, s.te, o);
     }
+    if (!far) lp_rescale(m, c, s.rest, s.te);
+    return s;
+  }
+};
+
+template <typename T, int THREADS, bool ENT, bool TOP, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS > 32 ? 32 : 1024 / THREADS) logprob_kernel(const LogprobArgs a) {
+  constexpr int kPiece = 16 / sizeof(T), kWarps = THREADS / 32;
+  constexpr int kPerGroup = THREADS <= kLpGroups ? 1 : THREADS / kLpGroups, kGroups = THREADS / kPerGroup;   // lanes of a group: 1, 2 or 4
+  __shared__ LpShared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0, ranks = CLUSTER ? static_cast<int>(cluster_size()) : 1;
+  const int step = static_cast<int>(gridDim.x) / ranks;
+  // rows without a target of which nothing else is asked are not read
+  auto next = [&](int row) {
+    if (!ENT && !TOP && a.targets) {
+      while (row < a.rows && a.targets[row] == a.ignore_index) {
+        if (rank == 0 && threadIdx.x == 0) {
+          a.logprob[row] = 0.f;
+          *reinterpret_cast<float2*>(a.stats + 2LL * row) = make_float2(-INFINITY, 0.f);
+        }
+        if (row >= a.rows - step) return a.rows;
+        row += step;
+      }
+    }
+    return row;
+  };
+  int row = next(static_cast<int>(blockIdx.x) / ranks);
+  LpSweep<T, THREADS> sweep;
+  uint4 cur[kLpChunk], other[kLpChunk];      // one is worked on while the other is loaded
+  bool flip = false;
+  if (row < a.rows) {
+    sweep.start(a.logits, lp_offset(a, row), a.vocab, rank, ranks);
+    sweep.load(0, a.vocab, cur);
+  }
+  int turn = 0;
+  while (row < a.rows) {
+    // what the first thread needs of the row beside its pieces
+    long long target = -1;
+    float at_target = 0.f;
+    if (a.targets && rank == 0 && threadIdx.x == 0) {
+      target = a.targets[row];
+      if (target >= 0 && target < a.vocab) at_target = lp_load(static_cast<const T*>(a.logits), lp_offset(a, row) + target);
+    }
+    const int upcoming = row >= a.rows - step ? a.rows : next(row + step);
+    // 1. the sums
+    LpRunning<T, ENT> sums;
+    sums.clear();
+    float mine = -INFINITY;
+    const int chunks = max(sweep.chunks, 1);             // an empty slice of a cluster still hands its loads on
+    auto chunk = [&](int k, const uint4 (&w)[kLpChunk], uint4 (&to_come)[kLpChunk]) {
+      if (k + 1 < chunks) {
+        sweep.load(k + 1, a.vocab, to_come);
+      } else if (upcoming < a.rows) {
+        sweep.start(a.logits, lp_offset(a, upcoming), a.vocab, rank, ranks);
+        sweep.load(0, a.vocab, to_come);
+      }
+      float most[kLpChunk];
+#pragma unroll
+      for (int i = 0; i < kLpChunk; ++i) most[i] = lp_piece_max<T>(w[i]);
+      const float largest = lp_max(lp_max(most[0], most[1]), lp_max(most[2], most[3]));
+      if (TOP) mine = lp_max(mine, largest);
+      sums.add(w, most, lp_warp_max(largest));
+    };
+    for (int k = 0; k < chunks; ++k) {
+      if (flip) chunk(k, other, cur);
+      else chunk(k, cur, other);
+      flip = !flip;
+    }
+    LpSums s = sums.warp_sums();
+    if (TOP) {
+      float group = mine;
+#pragma unroll
+      for (int o = 1; o < kPerGroup; o <<= 1) group = lp_max(group, __shfl_xor_sync(0xffffffffu, group, o));
+      if (threadIdx.x % kPerGroup == 0) reinterpret_cast<float*>(sh.group)[threadIdx.x / kPerGroup] = group;
+    }
     if (kWarps > 1 || TOP) {
       if (lane == 0) sh.part[turn][warp] = s;
       __syncthreads();
     }
-    if (warp == 0 && kWarps > 1) {
-      s.count = s.rest = s.te = 0.f;
-      if (lane < kWarps) s = sh.part[turn][lane];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        s.count += __shfl_xor_sync(0xffffffffu, s.count, o);
-        s.rest += __shfl_xor_sync(0xffffffffu, s.rest, o);
-        if (ENT) s.te += __shfl_xor_sync(0xffffffffu, s.te, o);
+    if (warp == 0) {
+      if (kWarps > 1) s = lp_join(sh.part[turn][lane < kWarps ? lane : 0], lane < kWarps);
+      if (!CLUSTER && lane == 0) {
+        const float2 mz = lp_finish(a, row, s, target, at_target);
+        if (TOP) sh.result = mz;
+      }
+      if (CLUSTER && lane == 0) {
+        const uint32_t to = in_first_cta(&sh.slice[turn][rank]);
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(s.m), "f"(s.count), "f"(s.rest), "f"(s.te) : "memory");
       }
     }
-    if (!CLUSTER && threadIdx.x == 0) {
-      const float2 mz = lp_finish(a, row, s, target, at_target);
-      if (TOP) sh.result = mz;
-    }
-    if (CLUSTER && threadIdx.x == 0) {
-      const uint32_t to = in_first_cta(&sh.slice[turn][rank]);
-      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(s.m), "f"(s.count), "f"(s.rest), "f"(s.te) : "memory");
-    }
-    // 3. the alternatives
+    // 2. the alternatives
     if (TOP) {
-      const float bound = sh.bound;
-      if (mine >= bound) {
+      // The bound: the group maximum that top - 1 others stand before.  kPerGroup threads per group, each counting in its
+      // share of the others.
+      {
+        const int g = threadIdx.x / kPerGroup, p = threadIdx.x % kPerGroup;
+        constexpr int kShare = kGroups / 4 / kPerGroup;
+        const float v = reinterpret_cast<const float*>(sh.group)[g];
+        int before = 0;
+#pragma unroll 4
+        for (int q = 0; q < kShare; ++q) {
+          const int j = p * kShare + q;
+          const float4 o = sh.group[j];
+          before += (o.x > v || (o.x == v && 4 * j < g)) + (o.y > v || (o.y == v && 4 * j + 1 < g)) +
+                    (o.z > v || (o.z == v && 4 * j + 2 < g)) + (o.w > v || (o.w == v && 4 * j + 3 < g));
+        }
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          if (!(lp_piece_max<T>(raw[i]) >= bound)) continue;
-          if (i * THREADS + static_cast<int>(threadIdx.x) >= now.pieces) continue;
-          uint4 w = raw[i];
-          const int e0 = (now.first + i * THREADS + static_cast<int>(threadIdx.x)) * kPiece - now.lead;
-#pragma unroll 1
-          for (int e = 0; e < kPiece; ++e) {                     // few pieces come here: element by element, shifted out below
-            const float v = sizeof(T) == 2 ? __uint_as_float(w.x << 16) : __uint_as_float(w.x);
-            if (v >= bound && e0 + e >= 0 && e0 + e < a.vocab) {
-              const int k = atomicAdd(&sh.found, 1);
-              if (k < kLpCandidates) sh.keys[k] = lp_key(v, e0 + e);
-            }
-            if (sizeof(T) == 2) {
-              w.x = w.x >> 16 | w.y << 16;
-              w.y = w.y >> 16 | w.z << 16;
-              w.z = w.z >> 16 | w.w << 16;
-              w.w >>= 16;
-            } else {
-              w.x = w.y; w.y = w.z; w.z = w.w;
-            }
-          }
+        for (int o = 1; o < kPerGroup; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+        if (p == 0 && before == a.top - 1) sh.bound = v;
+        if (threadIdx.x == 0) sh.hot = sh.found = 0;
+      }
+      __syncthreads();
+      const float bound = sh.bound;
+      if (mine >= bound) sh.hots[atomicAdd(&sh.hot, 1)] = static_cast<unsigned short>(threadIdx.x);
+      // a NaN anywhere in the slice: in a group's maximum, so in the first thread's count of them; its own test is cheaper
+      bool nan = false;
+      if (threadIdx.x < kGroups) nan = reinterpret_cast<const float*>(sh.group)[threadIdx.x] != reinterpret_cast<const float*>(sh.group)[threadIdx.x];
+      const bool slow_nan = __syncthreads_or(nan);
+      const LpRow r = lp_row<T>(a.logits, lp_offset(a, row), a.vocab, rank, ranks);
+      const int hot = sh.hot, sweeps = r.pieces > 0 ? (r.pieces + THREADS - 1) / THREADS : 0;
+      for (int k = threadIdx.x; k < hot * sweeps && !slow_nan; k += THREADS) {
+        const int piece = sh.hots[k % hot] + (k / hot) * THREADS;
+        if (piece >= r.pieces) continue;
+        const uint4 w = lp_fetch<T>(r, a.vocab, piece);
+        if (!(lp_piece_max<T>(w) >= bound)) continue;
+        float f[kPiece];
+        lp_unpack<T>(w, f);
+        uint32_t reach = 0;
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) reach |= f[e] >= bound ? 1u << e : 0u;
+        const int e0 = (r.first + piece) * kPiece - r.lead;
+        while (reach) {                                        // hardly ever more than one
+          const int e = __ffs(reach) - 1;
+          reach &= reach - 1;
+          if (e0 + e < 0 || e0 + e >= a.vocab) continue;
+          const int word = sizeof(T) == 2 ? e >> 1 : e;
+          const uint32_t bits = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
+          const float x = __uint_as_float(sizeof(T) == 4 ? bits : e & 1 ? bits & 0xffff0000u : bits << 16);
+          const int at = atomicAdd(&sh.found, 1);
+          if (at < kLpCandidates) sh.keys[at] = lp_key(x, e0 + e);
         }
       }
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (upcoming < a.rows) raw[i] = lp_fetch<T>(r, a.vocab, i * THREADS + threadIdx.x);
       __syncthreads();
       const int found = sh.found;
-      const bool slowly = found > kLpCandidates || m != m;
-      if (slowly) {
-        lp_pick_slowly<T>(now, a.vocab, a.top, sh.best, sh.picked);
-      } else {
-        if (threadIdx.x < 32) sh.picked[threadIdx.x] = 0;
-        __syncthreads();
-        for (int c = threadIdx.x; c < found; c += THREADS) {
-          const unsigned long long key = sh.keys[c];
-          int before = 0;
-          for (int j = 0; j < found; ++j) before += sh.keys[j] > key;
-          if (before < a.top) sh.picked[before] = key;
-        }
-        __syncthreads();
-      }
-      if (threadIdx.x == 0) sh.found = 0;
-      if (static_cast<int>(threadIdx.x) < a.top) {
-        const unsigned long long key = sh.picked[threadIdx.x];
+      auto put = [&](int place, unsigned long long key) {
         if (!CLUSTER) {
-          lp_put_top(a, row, threadIdx.x, key, sh.result);
+          sh.picked[place] = key;
         } else {
-          const uint32_t to = in_first_cta(&sh.slice_keys[turn][rank][threadIdx.x]);
+          const uint32_t to = in_first_cta(&sh.slice_keys[turn][rank][place]);
           asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(key) : "memory");
         }
+      };
+      if (found > kLpCandidates || slow_nan) {
+        lp_pick_slowly<T>(r, a.vocab, a.top, sh.best, sh.picked);
+        if (CLUSTER && static_cast<int>(threadIdx.x) < a.top) put(threadIdx.x, sh.picked[threadIdx.x]);
+      } else {
+        // eight threads per candidate count the ones before it
+        for (int c0 = 0; c0 < found; c0 += THREADS / 8) {
+          const int c = c0 + threadIdx.x / 8;
+          const unsigned long long key = c < found ? sh.keys[c] : 0;
+          int before = 0;
+          for (int j = threadIdx.x % 8; j < found; j += 8) before += sh.keys[j] > key;
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+          if (threadIdx.x % 8 == 0 && c < found && before < a.top) put(before, key);
+        }
+        if (CLUSTER && static_cast<int>(threadIdx.x) >= found && static_cast<int>(threadIdx.x) < a.top) put(threadIdx.x, 0);
+      }
+      if (!CLUSTER) {
+        __syncthreads();                     // the places, and the first thread's result
+        if (static_cast<int>(threadIdx.x) < a.top) lp_put_top(a, row, threadIdx.x, sh.picked[threadIdx.x], sh.result);
       }
     }
     if (CLUSTER) {
@@ -493,24 +620,37 @@ __global__ void __launch_bounds__(THREADS, THREADS > 512 ? 1 : 1024 / THREADS) l
       __syncwarp();
       cluster_barrier();
       if (rank == 0) {
-        if (!TOP) {
-          if (threadIdx.x == 0) lp_finish(a, row, lp_join(sh.slice[turn], ranks), target, at_target);
-        } else {
-          if (threadIdx.x == 0) sh.result = lp_finish(a, row, lp_join(sh.slice[turn], ranks), target, at_target);
+        if (warp == 0) {
+          const LpSums all = lp_join(sh.slice[turn][lane < ranks ? lane : 0], lane < ranks);
+          if (lane == 0) {
+            const float2 mz = lp_finish(a, row, all, target, at_target);
+            if (TOP) sh.result = mz;
+          }
+        }
+        if (TOP) {
           __syncthreads();
           const float2 mz = sh.result;
-          for (int c = threadIdx.x; c < ranks * a.top; c += THREADS) {
-            const unsigned long long key = sh.slice_keys[turn][c / a.top][c % a.top];
-            if (key == 0) continue;
+          const int all = ranks * a.top;
+          for (int c0 = 0; c0 < all; c0 += THREADS / 8) {
+            const int c = c0 + threadIdx.x / 8, q = threadIdx.x % 8;
+            const unsigned long long key = c < all ? sh.slice_keys[turn][c / a.top][c % a.top] : 0;
             int before = 0;
-            for (int q = 0; q < ranks; ++q)
-              for (int j = 0; j < a.top; ++j) before += sh.slice_keys[turn][q][j] > key;
-            if (before < a.top) lp_put_top(a, row, before, key, mz);
+            if (key != 0 && q < ranks) {
+              // a slice's keys descend: the ones before this one are its first ones
+              int end = a.top;
+              while (before < end) {
+                const int mid = (before + end) >> 1;
+                if (sh.slice_keys[turn][q][mid] > key) before = mid + 1;
+                else end = mid;
+              }
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+            if (q == 0 && key != 0 && before < a.top) lp_put_top(a, row, before, key, mz);
           }
         }
       }
     }
-    if (upcoming < a.rows) head(upcoming);
     row = upcoming;
     turn ^= 1;
   }
@@ -534,136 +674,164 @@ __device__ __forceinline__ void lp_store_piece<float>(void* p, const float (&f)[
   *static_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
 }
 
+// what a row's gradient is made of
 struct LpGrad {
-  float m, logz, whole, dh, h;
-  bool ent, none;
-  // the gradient of a token for which nothing arrives on its own
-  __device__ __forceinline__ float of(float x) const {
-    const float lp = (x - m) - logz, p = lp_exp2(lp * kLog2e);
-    const float g = -whole * p;
-    return ent ? (p == 0.f ? g : g - dh * p * (lp + h)) : g;
-  }
-  // ... and of one for which `share` does
-  __device__ __forceinline__ float of(float x, float share) const {
-    const float lp = (x - m) - logz, p = expf(lp);
-    const float g = (share - whole) * p - share * expm1f(lp);
-    return ent && p != 0.f ? g - dh * p * (lp + h) : g;
-  }
-};
+  float m, logz, whole, dh, h, dt;
+  int target;                    // -1: nothing arrives for it
+  float dk;                      // per lane: what arrives for its alternative
+  int index;                     // that alternative, -1 outside the vocabulary
+  bool zero;                     // nothing to read: the row is `fill`
+  float fill;
 
-// WARP: a warp takes whole rows (they are at most 32 * kLpPieces pieces and a ragged end); else gridDim covers rows * runs.
-template <typename T, bool WARP>
-__global__ void __launch_bounds__(256) logprob_bwd_kernel(const LogprobBwdArgs a, int runs) {
-  constexpr int kPiece = 16 / sizeof(T), kWidth = WARP ? 32 : 256;
-  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const long long total = a.rows * runs, step = static_cast<long long>(gridDim.x) * (WARP ? 8 : 1);
-  for (long long work = WARP ? static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x; work < total; work += step) {
-    const long long row = WARP ? work : work / runs;
-    const int run = WARP ? 0 : static_cast<int>(work - row * runs);
-    const long long batch = row / a.seq;
-    const T* x = static_cast<const T*>(a.logits) + batch * a.batch_stride + (row - batch * a.seq) * a.row_stride;
-    T* out = static_cast<T*>(a.grad) + row * a.vocab;
-    // the row's numbers; what arrives for the alternatives, one per lane
-    const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * row);
-    LpGrad g = {st.x, st.y, 0.f, 0.f, 0.f, a.d_entropy != nullptr, st.x == -INFINITY};
-    if (a.d_entropy) { g.dh = a.d_entropy[row]; g.h = a.entropy[row]; }
-    long long target = -1;
-    float dt = 0.f;
+  __device__ __forceinline__ void load(const LogprobBwdArgs& a, int row) {
+    const float2 st = *reinterpret_cast<const float2*>(a.stats + 2LL * row);
+    m = st.x;
+    logz = st.y;
+    dh = h = dt = dk = 0.f;
+    if (a.d_entropy) { dh = a.d_entropy[row]; h = a.entropy[row]; }
+    target = index = -1;
     if (a.d_logprob) {
-      target = a.targets[row];
-      if (target == a.ignore_index) {
-        target = -1;
-      } else {
-        dt = target >= 0 && target < a.vocab ? a.d_logprob[row] : NAN;
+      const long long t = a.targets[row];
+      const float d = a.d_logprob[row];
+      if (t != a.ignore_index) {
+        const bool in = t >= 0 && t < a.vocab;
+        target = in ? static_cast<int>(t) : -1;
+        dt = in ? d : NAN;
       }
     }
     const int lane = threadIdx.x & 31;
-    float dk = 0.f;
-    long long index = -1;
-    if (lane < a.top) { dk = a.d_top[row * a.top + lane]; index = a.top_index[row * a.top + lane]; }
-    g.whole = dk;
+    if (lane < a.top) {
+      dk = a.d_top[static_cast<long long>(row) * a.top + lane];
+      const long long t = a.top_index[static_cast<long long>(row) * a.top + lane];
+      index = t >= 0 && t < a.vocab ? static_cast<int>(t) : -1;
+    }
+  }
+  // once the loads are in; all threads of a warp
+  __device__ __forceinline__ void ready(const LogprobBwdArgs& a) {
+    whole = dk;
     if (a.top) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) g.whole += __shfl_xor_sync(0xffffffffu, g.whole, o);
+      for (int o = 16; o > 0; o >>= 1) whole += __shfl_xor_sync(0xffffffffu, whole, o);
     }
-    g.whole += dt;
-    const bool zero = g.none || (g.whole == 0.f && !a.top && !g.ent);        // nothing to read
-    const float fill = g.whole == g.whole ? 0.f : NAN;
-    // pieces counted from the aligned address at or below the row's start, if x and out lie alike
-    const int phase = static_cast<int>(reinterpret_cast<uintptr_t>(out) & 15u), lead = phase / static_cast<int>(sizeof(T));
-    const bool alike = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15u) == phase;
-    const int pieces = (lead + a.vocab + kPiece - 1) / kPiece;
-    const int first = run * (kWidth * kLpPieces), last = min(pieces, WARP ? pieces : first + kWidth * kLpPieces);
-    for (int p0 = first; p0 < last; p0 += kWidth * kLpPieces) {
-      uint4 raw[kLpPieces];
+    whole += dt;
+    zero = m == -INFINITY || (whole == 0.f && !a.top && !a.d_entropy);
+    fill = whole == whole ? 0.f : NAN;
+  }
+  // the gradient of two tokens for which nothing arrives on its own
+  template <bool ENT>
+  __device__ __forceinline__ f32x2 of(f32x2 x) const {
+    const f32x2 d = f2_add(x, f2_make(-m, -m));
+    f32x2 lp = 0;
+    float u0, u1;
+    if (ENT) {
+      lp = f2_add(d, f2_make(-logz, -logz));
+      f2_split(f2_mul(lp, f2_make(kLog2e, kLog2e)), u0, u1);
+    } else {
+      f2_split(f2_fma(d, f2_make(kLog2e, kLog2e), f2_make(-logz * kLog2e, -logz * kLog2e)), u0, u1);
+    }
+    const f32x2 p = f2_make(lp_exp2(u0), lp_exp2(u1));
+    if (!ENT) return f2_mul(p, f2_make(-whole, -whole));
+    // p (-whole - dh (lp + h)): p is 0 long before lp is -10000: the bracket stays finite, a NaN stays one
+    float l0, l1;
+    f2_split(lp, l0, l1);
+    lp = f2_make(lp_max(l0, -10000.f), lp_max(l1, -10000.f));
+    return f2_mul(p, f2_fma(f2_add(lp, f2_make(h, h)), f2_make(-dh, -dh), f2_make(-whole, -whole)));
+  }
+  template <bool ENT>
+  __device__ __forceinline__ float of(float x) const {
+    float lo, hi;
+    f2_split(of<ENT>(f2_make(x, x)), lo, hi);
+    return lo;
+  }
+  // ... and of one for which `share` does
+  template <bool ENT>
+  __device__ __forceinline__ float of(float x, float share) const {
+    const float lp = (x - m) - logz, p = expf(lp);
+    const float g = (share - whole) * p - share * expm1f(lp);
+    return ENT && p != 0.f ? g - dh * p * (lp + h) : g;
+  }
+};
+
+// A warp takes a whole short row (WARP), a CTA one run of kWidth * kLpPieces pieces of a longer one.
+template <typename T, bool WARP, bool ENT>
+__global__ void __launch_bounds__(256) logprob_bwd_kernel(const LogprobBwdArgs a) {
+  constexpr int kPiece = 16 / sizeof(T), kWidth = WARP ? 32 : 256;
+  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int row = WARP ? static_cast<int>(blockIdx.x * 8 + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x), run = WARP ? 0 : blockIdx.y;
+  if (WARP && (row >= a.rows || row < 0)) return;
+  const T* x = static_cast<const T*>(a.logits) + lp_offset(a, row);
+  T* out = static_cast<T*>(a.grad) + static_cast<long long>(row) * a.vocab;
+  LpGrad g;
+  g.load(a, row);
+  // pieces counted from the aligned address at or below the row's start, if x and out lie alike
+  const int phase = static_cast<int>(reinterpret_cast<uintptr_t>(out) & 15u), lead = phase / static_cast<int>(sizeof(T));
+  const bool alike = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15u) == phase;
+  const int first = run * (kWidth * kLpPieces), last = min((lead + a.vocab + kPiece - 1) / kPiece, first + kWidth * kLpPieces);
+  g.ready(a);
+  uint4 raw[kLpPieces];
 #pragma unroll
-      for (int i = 0; i < kLpPieces; ++i) {
-        const int piece = p0 + i * kWidth + t, e0 = piece * kPiece - lead;
-        if (piece < last && alike && !zero && e0 >= 0 && e0 + kPiece <= a.vocab) raw[i] = load16_stream(x + e0);
-      }
+  for (int i = 0; i < kLpPieces; ++i) {
+    const int piece = first + i * kWidth + t, e0 = piece * kPiece - lead;
+    if (piece < last && alike && !g.zero && e0 >= 0 && e0 + kPiece <= a.vocab) raw[i] = load16_stream(x + e0);
+  }
 #pragma unroll
-      for (int i = 0; i < kLpPieces; ++i) {
-        const int piece = p0 + i * kWidth + t, e0 = piece * kPiece - lead;
-        if (piece >= last) continue;
-        if (e0 >= 0 && e0 + kPiece <= a.vocab) {
-          float f[kPiece];
-          if (zero) {
+  for (int i = 0; i < kLpPieces; ++i) {
+    const int piece = first + i * kWidth + t, e0 = piece * kPiece - lead;
+    if (piece >= last) continue;
+    if (alike && e0 >= 0 && e0 + kPiece <= a.vocab) {
+      float f[kPiece];
+      if (g.zero) {
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) f[e] = fill;
-          } else {
-            if (alike) {
-              lp_unpack<T>(raw[i], f);
-            } else {
+        for (int e = 0; e < kPiece; ++e) f[e] = g.fill;
+      } else {
+        lp_unpack<T>(raw[i], f);
+        const int hot = g.target - e0;
+        const bool has = !a.top && hot >= 0 && hot < kPiece;
+        float there = 0.f;
+        if (has) {
 #pragma unroll
-              for (int e = 0; e < kPiece; ++e) f[e] = lp_load(x, e0 + e);
-            }
-            const long long hot = target - e0;
-            const bool has = !a.top && hot >= 0 && hot < kPiece;
-            float there = 0.f;
-            if (has) {
+          for (int e = 0; e < kPiece; ++e) there = e == hot ? f[e] : there;
+          there = g.of<ENT>(there, g.dt);
+        }
 #pragma unroll
-              for (int e = 0; e < kPiece; ++e) there = e == static_cast<int>(hot) ? f[e] : there;
-              there = g.of(there, dt);
-            }
+        for (int e = 0; e < kPiece; e += 2) f2_split(g.of<ENT>(f2_make(f[e], f[e + 1])), f[e], f[e + 1]);
+        if (has) {
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) f[e] = g.of(f[e]);
-            if (has) {
-#pragma unroll
-              for (int e = 0; e < kPiece; ++e) f[e] = e == static_cast<int>(hot) ? there : f[e];
-            }
-          }
-          lp_store_piece<T>(out + e0, f);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kPiece; ++e) {
-            const int c = e0 + e;
-            if (c < 0 || c >= a.vocab) continue;
-            out[c] = T(zero ? fill : c == target && !a.top ? g.of(lp_load(x, c), dt) : g.of(lp_load(x, c)));
-          }
+          for (int e = 0; e < kPiece; ++e) f[e] = e == hot ? there : f[e];
         }
       }
-    }
-    if (a.top && !zero) {
-      // the tokens for which something arrives: the alternatives, and the target behind them, one per lane and each by its
-      // first mention; every warp of a CTA knows them, the first one writes those of the CTA's run
-      if (WARP) __syncwarp();
-      else __syncthreads();
-      if (WARP || threadIdx.x < 32) {
-        const int from = first * kPiece - lead, to = last * kPiece - lead;
-        float share = 0.f, target_share = dt;
-        bool seen = false, target_seen = false;
-        for (int j = 0; j < a.top; ++j) {
-          const long long o = __shfl_sync(0xffffffffu, index, j);
-          const float d = __shfl_sync(0xffffffffu, dk, j);
-          if (o == index) { share += d; seen |= j < lane; }
-          if (o == target) { target_share += d; target_seen = true; }
-        }
-        if (index == target) share += dt;
-        if (lane < a.top && !seen && index >= 0 && index < a.vocab && index >= from && index < to)
-          out[index] = T(g.of(lp_load(x, index), share));
-        if (lane == 0 && !target_seen && target >= 0 && target < a.vocab && target >= from && target < to)
-          out[target] = T(g.of(lp_load(x, target), target_share));
+      lp_store_piece<T>(out + e0, f);
+    } else {
+      // a row's ragged end, or rows of x and out that lie differently
+#pragma unroll 1
+      for (int e = 0; e < kPiece; ++e) {
+        const int c = e0 + e;
+        if (c < 0 || c >= a.vocab) continue;
+        float v = g.fill;
+        if (!g.zero) v = c == g.target && !a.top ? g.of<ENT>(lp_load(x, c), g.dt) : g.of<ENT>(lp_load(x, c));
+        out[c] = T(v);
       }
+    }
+  }
+  if (a.top && !g.zero) {
+    // the tokens for which something arrives: the alternatives, and the target behind them, one per lane and each by its
+    // first mention; every warp of a CTA knows them, the first one writes those of the CTA's run
+    if (WARP) __syncwarp();
+    else __syncthreads();
+    if (WARP || threadIdx.x < 32) {
+      const int lane = threadIdx.x & 31, from = first * kPiece - lead, to = last * kPiece - lead;
+      float share = 0.f, target_share = g.dt;
+      bool seen = false, target_seen = false;
+      for (int j = 0; j < a.top; ++j) {
+        const int o = __shfl_sync(0xffffffffu, g.index, j);
+        const float d = __shfl_sync(0xffffffffu, g.dk, j);
+        if (o == g.index) { share += d; seen |= j < lane; }
+        if (o == g.target) { target_share += d; target_seen = true; }
+      }
+      if (g.index == g.target) share += g.dt;
+      if (lane < a.top && !seen && g.index >= 0 && g.index >= from && g.index < to) out[g.index] = T(g.of<ENT>(lp_load(x, g.index), share));
+      if (lane == 0 && !target_seen && g.target >= 0 && g.target >= from && g.target < to)
+        out[g.target] = T(g.of<ENT>(lp_load(x, g.target), target_share));
     }
   }
 }
@@ -699,15 +867,16 @@ template <typename T, int THREADS, bool ENT, bool TOP, bool CLUSTER>
 static int run_logprob(const LogprobArgs& a, int ranks, cudaStream_t stream) {
   auto kernel = logprob_kernel<T, THREADS, ENT, TOP, CLUSTER>;
   static PerDevice resident[4];            // by cluster size
-  const long long most = resident[ranks == 8 ? 3 : ranks >> 1].get([&] { return resident_clusters(kernel, THREADS, ranks); }), clusters = a.rows < most ? a.rows : most;
+  const long long most = resident[ranks == 8 ? 3 : ranks >> 1].get([&] { return resident_clusters(kernel, THREADS, ranks); });
+  const long long clusters = a.rows < most ? a.rows : most;
   cudaError_t e;
   if (CLUSTER) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = ranks; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(clusters * ranks)); cfg.blockDim = dim3(THREADS); cfg.stream = stream;
-    cfg.attrs = &attr; cfg.numAttrs = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * ranks)); cfg.blockDim = dim3(THREADS);
+    cfg.stream = stream; cfg.attrs = &attr; cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, kernel, a);
   } else {
     kernel<<<static_cast<unsigned>(clusters), THREADS, 0, stream>>>(a);
@@ -723,32 +892,33 @@ static int pick_logprob(const LogprobArgs& a, int ranks, cudaStream_t stream) {
   return a.entropy ? run_logprob<T, THREADS, true, false, CLUSTER>(a, ranks, stream) : run_logprob<T, THREADS, false, false, CLUSTER>(a, ranks, stream);
 }
 
-// The smallest CTA, then the smallest cluster, whose registers hold a row (one piece more than its bytes, where it starts
-// inside a piece).
+// Short rows: smaller CTAs, at least two chunks for each.  Few long rows are spread over clusters, as far as a slice keeps two
+// chunks and the SMs' places for CTAs go.
 template <typename T>
 static int launch_logprob(const LogprobArgs& a, cudaStream_t stream) {
-  const int pieces = static_cast<int>((static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16) + 1;
-  if (pieces <= 32 * 8) return pick_logprob<T, 32, false>(a, 1, stream);
-  if (pieces <= 64 * 8) return pick_logprob<T, 64, false>(a, 1, stream);
-  if (pieces <= 128 * 8) return pick_logprob<T, 128, false>(a, 1, stream);
-  if (pieces <= 256 * 8) return pick_logprob<T, 256, false>(a, 1, stream);
-  if (pieces <= 512 * 8) return pick_logprob<T, 512, false>(a, 1, stream);
-  for (int ranks = 2; ranks <= 8; ranks *= 2)
-    if (pieces <= ranks * 512 * 8) return pick_logprob<T, 512, true>(a, ranks, stream);
-  return pick_logprob<T, 576, true>(a, 8, stream);
+  const long long pieces = (static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1;
+  int ranks = 1;
+  while (ranks < 8 && static_cast<long long>(a.rows) * ranks * 2 <= sm_count() * LPA && pieces / (ranks * 2) >= LPM) ranks *= 2;
+  if (ranks > 1) return pick_logprob<T, 256, true>(a, ranks, stream);
+  if (pieces <= 2 * 32 * kLpChunk) return pick_logprob<T, 32, false>(a, 1, stream);
+  if (pieces <= 2 * 64 * kLpChunk) return pick_logprob<T, 64, false>(a, 1, stream);
+  if (pieces <= 2 * 128 * kLpChunk) return pick_logprob<T, 128, false>(a, 1, stream);
+  return pick_logprob<T, 256, false>(a, 1, stream);
+}
+
+template <typename T, bool WARP, bool ENT>
+static void run_logprob_bwd(const LogprobBwdArgs& a, int runs, cudaStream_t stream) {
+  if (WARP) logprob_bwd_kernel<T, WARP, ENT><<<static_cast<unsigned>((a.rows + 7LL) / 8), 256, 0, stream>>>(a);
+  else logprob_bwd_kernel<T, WARP, ENT><<<dim3(a.rows, runs), 256, 0, stream>>>(a);
 }
 
 template <typename T>
 static int launch_logprob_bwd(const LogprobBwdArgs& a, cudaStream_t stream) {
   const long long pieces = (static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1;
-  if (pieces <= 2 * 32 * kLpPieces) {
-    const long long blocks = (a.rows + 7) / 8;
-    logprob_bwd_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a, 1);
-  } else {
-    const int runs = static_cast<int>((pieces + 256 * kLpPieces - 1) / (256 * kLpPieces));
-    const long long total = a.rows * runs;
-    logprob_bwd_kernel<T, false><<<static_cast<unsigned>(total < 0x7fffffffLL ? total : 0x7fffffffLL), 256, 0, stream>>>(a, runs);
-  }
+  const bool warp = pieces <= 32 * kLpPieces;                       // short rows: a warp each
+  const int width = (warp ? 32 : 256) * kLpPieces, runs = static_cast<int>((pieces + width - 1) / width);
+  if (warp) a.d_entropy ? run_logprob_bwd<T, true, true>(a, runs, stream) : run_logprob_bwd<T, true, false>(a, runs, stream);
+  else a.d_entropy ? run_logprob_bwd<T, false, true>(a, runs, stream) : run_logprob_bwd<T, false, false>(a, runs, stream);
   HYC_LAUNCHED();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? HYC_OK : cuda_fail(e, "logprob_bwd_kernel");
@@ -773,7 +943,8 @@ int hyc_token_logprobs(const hyc_logprob_args* q, void* stream_) {
       lp_misaligned(q->entropy, 4) || lp_misaligned(q->stats, 8) || lp_misaligned(q->top_logprob, 4) || lp_misaligned(q->top_index, 8))
     return HYC_ERR_ALIGN;
   LogprobArgs a;
-  a.logits = q->logits; a.rows = q->rows; a.row_stride = q->row_stride; a.batch_stride = q->batch_stride; a.seq = q->seq;
+  a.logits = q->logits; a.row_stride = q->row_stride; a.batch_stride = q->batch_stride;
+  a.rows = static_cast<int>(q->rows); a.seq = static_cast<int>(q->seq < 0x7fffffffLL ? q->seq : 0x7fffffffLL);
   a.vocab = q->vocab; a.top = q->top; a.targets = reinterpret_cast<const long long*>(q->targets); a.ignore_index = q->ignore_index;
   a.logprob = q->logprob; a.entropy = q->entropy; a.stats = q->stats; a.top_logprob = q->top_logprob;
   a.top_index = reinterpret_cast<long long*>(q->top_index);
@@ -795,7 +966,8 @@ int hyc_token_logprobs_bwd(const hyc_logprob_bwd_args* q, void* stream_) {
       lp_misaligned(q->top_index, 8))
     return HYC_ERR_ALIGN;
   LogprobBwdArgs a;
-  a.logits = q->logits; a.rows = q->rows; a.row_stride = q->row_stride; a.batch_stride = q->batch_stride; a.seq = q->seq;
+  a.logits = q->logits; a.row_stride = q->row_stride; a.batch_stride = q->batch_stride;
+  a.rows = static_cast<int>(q->rows); a.seq = static_cast<int>(q->seq < 0x7fffffffLL ? q->seq : 0x7fffffffLL);
   a.vocab = q->vocab; a.top = q->d_top ? q->top : 0; a.targets = reinterpret_cast<const long long*>(q->targets);
   a.ignore_index = q->ignore_index; a.stats = q->stats; a.entropy = q->entropy; a.d_logprob = q->d_logprob;
   a.d_entropy = q->d_entropy; a.d_top = q->d_top; a.top_index = reinterpret_cast<const long long*>(q->top_index); a.grad = q->grad;

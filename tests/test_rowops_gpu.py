@@ -565,8 +565,11 @@ def test_logprobs_beyond_32_bit_offsets(ops):
     g = ops.token_logprobs_bwd(big, stats, tt, torch.ones(rows, device="cuda"))
     _near(g[-3:], *ro.token_logprobs_bwd(x, out.stats.cpu(), t, torch.ones(3)))
     assert int(torch.count_nonzero(g[:-3])) == 0
+    # three rows are spread over clusters, 140000 are not: the sums run in another order, each within the counted roundings
     again = ops.token_logprobs(big, tt)
-    assert torch.equal(again.stats[-3:], out.stats)
+    want, bound = ro.token_logprobs(x, t)
+    _near(again.stats[-3:], want["stats"], bound["stats"])
+    _near(again.logprob[-3:], want["logprob"], bound["logprob"])
 
 
 def test_logprobs_of_no_rows_and_of_one_vector(ops):
