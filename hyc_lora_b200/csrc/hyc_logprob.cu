@@ -10,10 +10,6 @@
 
 #include "hyc_host.cuh"
 
-#ifndef LPM
-#define LPM 512
-#define LPA 4
-#endif
 namespace hyc {
 
 struct LogprobArgs {
@@ -89,7 +85,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 //
 // Issue slots are as scarce as bytes here: bf16 leaves 11 of them per 32 elements at full bandwidth, and the exponentials take
 // 8 of their unit's cycles.  Holding whole rows in registers instead, with a barrier behind the maximum and one behind the
-// sums, took 122 us at 8192 x 32000 (512 threads of 8 pieces) or 186 (256 of 16); staging them in shared memory 151.
+// sums, took 122 us at 8192 x 32000 (512 threads of 8 pieces) or 186 (256 of 16), staging them in shared memory 151; this takes 104.
+// Chunks of 2 pieces take 107, of 6 113; two buffers that change places instead of a copy 114 (spills).
 constexpr int kLpCandidates = 256, kLpGroups = 64, kLpChunk = 4;
 
 struct alignas(16) LpSums {        // stored by 16 bytes into another CTA's shared memory
@@ -446,7 +443,7 @@ struct LpRunning {
 };
 
 template <typename T, int THREADS, bool ENT, bool TOP, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS > 32 ? 32 : 1024 / THREADS) logprob_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(THREADS, 768 / THREADS > 24 ? 24 : 768 / THREADS) logprob_kernel(const LogprobArgs a) {
   constexpr int kPiece = 16 / sizeof(T), kWarps = THREADS / 32;
   constexpr int kPerGroup = THREADS <= kLpGroups ? 1 : THREADS / kLpGroups, kGroups = THREADS / kPerGroup;   // lanes of a group: 1, 2 or 4
   __shared__ LpShared sh;
@@ -469,8 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS > 32 ? 32 : 1024 / THR
   };
   int row = next(static_cast<int>(blockIdx.x) / ranks);
   LpSweep<T, THREADS> sweep;
-  uint4 cur[kLpChunk], other[kLpChunk];      // one is worked on while the other is loaded
-  bool flip = false;
+  uint4 cur[kLpChunk];
   if (row < a.rows) {
     sweep.start(a.logits, lp_offset(a, row), a.vocab, rank, ranks);
     sweep.load(0, a.vocab, cur);
@@ -500,14 +496,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS > 32 ? 32 : 1024 / THR
       float most[kLpChunk];
 #pragma unroll
       for (int i = 0; i < kLpChunk; ++i) most[i] = lp_piece_max<T>(w[i]);
-      const float largest = lp_max(lp_max(most[0], most[1]), lp_max(most[2], most[3]));
+      float largest = most[0];
+#pragma unroll
+      for (int i = 1; i < kLpChunk; ++i) largest = lp_max(largest, most[i]);
       if (TOP) mine = lp_max(mine, largest);
       sums.add(w, most, lp_warp_max(largest));
     };
     for (int k = 0; k < chunks; ++k) {
-      if (flip) chunk(k, other, cur);
-      else chunk(k, cur, other);
-      flip = !flip;
+      uint4 w[kLpChunk];
+#pragma unroll
+      for (int i = 0; i < kLpChunk; ++i) w[i] = cur[i];
+      chunk(k, w, cur);
     }
     LpSums s = sums.warp_sums();
     if (TOP) {
@@ -898,7 +897,7 @@ template <typename T>
 static int launch_logprob(const LogprobArgs& a, cudaStream_t stream) {
   const long long pieces = (static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1;
   int ranks = 1;
-  while (ranks < 8 && static_cast<long long>(a.rows) * ranks * 2 <= sm_count() * LPA && pieces / (ranks * 2) >= LPM) ranks *= 2;
+  while (ranks < 8 && static_cast<long long>(a.rows) * ranks * 2 <= sm_count() * 4 && pieces / (ranks * 2) >= 512) ranks *= 2;
   if (ranks > 1) return pick_logprob<T, 256, true>(a, ranks, stream);
   if (pieces <= 2 * 32 * kLpChunk) return pick_logprob<T, 32, false>(a, 1, stream);
   if (pieces <= 2 * 64 * kLpChunk) return pick_logprob<T, 64, false>(a, 1, stream);

@@ -8,7 +8,6 @@ dimensions are rows; rows may lie apart (a slice of a wider tensor), elements of
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 from typing import NamedTuple, Optional
 
@@ -33,22 +32,42 @@ class TokenLogprobs(NamedTuple):
     stats: torch.Tensor                   # fp32 [rows, 2]: largest logit, log of the sum of exp(x - largest)
 
 
-_NO_GUARD = contextlib.nullcontext()
+# The small calls of this module are bound by their host side: the raw-stream and device queries below are torch's cheap ones
+# (0.1 us each instead of 2.2 for a Stream object), and allocations of one dimension go through empty_strided (1.5 us, not 2.3).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _on(device: torch.device):
-    """Makes ``device`` current while a kernel is enqueued, where it is not already."""
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _stream(device: torch.device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _same_device(first: torch.Tensor, *others):
+def _device_of(first: torch.Tensor, *others) -> int:
+    """The index of the one CUDA device that all tensors are on."""
+    index = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
+            _require_cuda(first, t)
             raise RuntimeError(f"all tensors must be on one device, got {first.device} and {t.device}")
+    if index < 0:
+        _require_cuda(first)
+    return index
+
+
+def _launch(entry, name: str, args, index: int):
+    """Enqueues on the current stream of device ``index``, which is made current for the call where it is not."""
+    if index == _current_device():
+        code = entry(C.byref(args), _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = entry(C.byref(args), _raw_stream(index))
+    if code:
+        check(code, name)
+
+
+def _vector(n: int, dtype: torch.dtype, device) -> torch.Tensor:
+    return torch.empty_strided((n,), (1,), dtype=dtype, device=device)
+
+
+def _result(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor like ``x``."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _at(t: Optional[torch.Tensor]):
@@ -99,10 +118,14 @@ def rng_take(state: torch.Tensor) -> torch.Tensor:
     """A fresh ``(seed, call)`` pair from ``state`` (int64 [2] on the device), whose call number moves on by one.  Concurrent
     calls take different numbers, and so does every replay of a graph this was recorded into."""
     _check_rng(state)
-    _require_cuda(state)
-    used = torch.empty(2, dtype=torch.int64, device=state.device)
-    with _on(state.device):
-        check(lib.hyc_rng_take(state.data_ptr(), used.data_ptr(), _stream(state.device)), "hyc_rng_take")
+    index = _device_of(state)
+    used = torch.empty_like(state)
+    if index == _current_device():
+        code = lib.hyc_rng_take(state.data_ptr(), used.data_ptr(), _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = lib.hyc_rng_take(state.data_ptr(), used.data_ptr(), _raw_stream(index))
+    check(code, "hyc_rng_take")
     return used
 
 
@@ -110,8 +133,7 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: Optional[tor
     """``residual + dropout(x)``: element i (row-major) is kept where word i of the generator is at least ``p``, and divided by
     ``1 - p``.  The backward pass is the same call on the gradient, without residual, with the same ``rng``."""
     _check_rng(rng)
-    _require_cuda(x, rng, residual)
-    _same_device(x, rng, residual)
+    index = _device_of(x, rng, residual)
     if x.dim() == 0:
         raise ValueError("dropout takes tensors of at least one dimension")
     a = HycDropoutArgs()
@@ -129,10 +151,9 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: Optional[tor
         x, a.x_stride = _rows(x)
         a.cols = x.shape[-1]
         a.rows = x.numel() // max(1, a.cols)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _result(x)
     a.x, a.y, a.rng, a.p = x.data_ptr(), y.data_ptr(), rng.data_ptr(), p
-    with _on(x.device):
-        check(lib.hyc_dropout(C.byref(a), _stream(x.device)), "hyc_dropout")
+    _launch(lib.hyc_dropout, "hyc_dropout", a, index)
     return y
 
 
@@ -141,7 +162,7 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: Optional[tor
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5, *,
                residual: Optional[torch.Tensor] = None, p: float = 0.0, rng: Optional[torch.Tensor] = None) -> LayerNormOut:
     """Layer norm over the last dimension of ``residual + dropout(x)``; ``rng`` is needed where ``p > 0``."""
-    _require_cuda(x, weight, bias, residual, rng if p > 0.0 else None)
+    index = _device_of(x, weight, bias, residual, rng if p > 0.0 else None)
     if x.dim() == 0:
         raise ValueError("layer_norm takes tensors of at least one dimension")
     cols = x.shape[-1]
@@ -152,23 +173,20 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
     if p > 0.0:
         _check_rng(rng)
         a.rng = rng.data_ptr()
-    _same_device(x, weight, bias, residual, rng if p > 0.0 else None)
     if residual is not None:
         _like("residual", residual, x)
         residual, a.residual_stride = _rows(residual)
         a.residual = residual.data_ptr()
     x, a.x_stride = _rows(x)
     rows = x.numel() // max(1, cols)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _result(x)
     z = torch.empty_like(y) if residual is not None or p > 0.0 else None
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
+    mean = _vector(rows, torch.float32, x.device)
+    rstd = torch.empty_like(mean)
     a.rows, a.cols, a.eps, a.p = rows, cols, eps, p
     a.x, a.weight, a.bias, a.y, a.z = x.data_ptr(), _at(weight), _at(bias), y.data_ptr(), _at(z)
-    a.mean = stats.data_ptr()
-    a.rstd = a.mean + 4 * rows if rows else a.mean
-    with _on(x.device):
-        check(lib.hyc_layer_norm(C.byref(a), _stream(x.device)), "hyc_layer_norm")
+    a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
+    _launch(lib.hyc_layer_norm, "hyc_layer_norm", a, index)
     return LayerNormOut(y, x if z is None else z, mean, rstd)
 
 
@@ -178,8 +196,7 @@ def layer_norm_bwd(dy: torch.Tensor, z: torch.Tensor, weight: Optional[torch.Ten
     """``(dx, dresidual, dweight, dbias)`` of :func:`layer_norm`.  ``dz`` is a gradient that reaches the sum past the norm.
     Where ``p == 0`` dx and dresidual are one tensor.  dweight and dbias come in the weight's dtype (``param_dtype``, then
     the input's, where there is no weight)."""
-    _require_cuda(dy, z, weight, mean, rstd, dz, rng if p > 0.0 else None)
-    _same_device(dy, z, weight, mean, rstd, dz, rng if p > 0.0 else None)
+    index = _device_of(dy, z, weight, mean, rstd, dz, rng if p > 0.0 else None)
     if dy.dim() == 0:
         raise ValueError("layer_norm_bwd takes tensors of at least one dimension")
     cols = dy.shape[-1]
@@ -188,7 +205,7 @@ def layer_norm_bwd(dy: torch.Tensor, z: torch.Tensor, weight: Optional[torch.Ten
     a = HycLayerNormBwdArgs()
     a.dtype = _dtype_code(dy)
     kind = weight.dtype if weight is not None else param_dtype or dy.dtype
-    a.param_dtype = _dtype_code(torch.empty(0, dtype=kind)) if weight is None else _dtype_code(weight)
+    a.param_dtype = _dtype_code(torch.empty(0, dtype=kind)) if weight is None and kind != dy.dtype else _dtype_code(weight) if weight is not None else a.dtype
     if p > 0.0:
         _check_rng(rng)
         a.rng = rng.data_ptr()
@@ -201,21 +218,23 @@ def layer_norm_bwd(dy: torch.Tensor, z: torch.Tensor, weight: Optional[torch.Ten
     rows = dy.numel() // max(1, cols)
     _check_row_stats("mean", mean, rows)
     _check_row_stats("rstd", rstd, rows)
-    dresidual = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    dresidual = _result(dy)
     dx = torch.empty_like(dresidual) if p > 0.0 else dresidual
-    dweight = torch.empty(cols, dtype=kind, device=dy.device) if need_dweight else None
-    dbias = torch.empty(cols, dtype=kind, device=dy.device) if need_dbias else None
-    partials = None
+    dweight = dbias = partials = None
+    if need_dweight:
+        dweight = torch.empty_like(weight) if weight is not None else _vector(cols, kind, dy.device)
+    if need_dbias:
+        dbias = torch.empty_like(weight) if weight is not None else _vector(cols, kind, dy.device)
     if need_dweight or need_dbias:
         floats = lib.hyc_layer_norm_bwd_scratch_floats(rows, cols)
-        check(min(0, floats), "hyc_layer_norm_bwd_scratch_floats")
-        partials = torch.empty(floats, dtype=torch.float32, device=dy.device)
+        if floats < 0:
+            check(floats, "hyc_layer_norm_bwd_scratch_floats")
+        partials = _vector(floats, torch.float32, dy.device)
     a.rows, a.cols, a.p = rows, cols, p
     a.dy, a.z, a.weight, a.mean, a.rstd = dy.data_ptr(), z.data_ptr(), _at(weight), mean.data_ptr(), rstd.data_ptr()
     a.dresidual, a.dx = dresidual.data_ptr(), dx.data_ptr() if p > 0.0 else None
     a.dweight, a.dbias, a.partials = _at(dweight), _at(dbias), _at(partials)
-    with _on(dy.device):
-        check(lib.hyc_layer_norm_bwd(C.byref(a), _stream(dy.device)), "hyc_layer_norm_bwd")
+    _launch(lib.hyc_layer_norm_bwd, "hyc_layer_norm_bwd", a, index)
     return dx, dresidual, dweight, dbias
 
 
@@ -249,32 +268,38 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
 
     A target of ``ignore_index`` gives 0; where neither entropy nor alternatives are asked for its row is not read at all.  Any
     other target outside the vocabulary gives NaN.  A row without any finite logit (all -inf) gives -inf and entropy 0."""
-    _require_cuda(logits, targets)
-    _same_device(logits, targets)
+    device = _device_of(logits, targets)
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise ValueError("logits must have a last dimension of at least one value")
     a = HycLogprobArgs()
     a.dtype = _dtype_code(logits)
     lead, dev = logits.shape[:-1], logits.device
-    logprob = None
+    flat = len(lead) == 1
+
+    def per_row():
+        return _vector(lead[0], torch.float32, dev) if flat else torch.empty(lead, dtype=torch.float32, device=dev)
+
+    logprob = h = index = best = None
     if targets is not None:
         targets = _check_targets(logits, targets)
-        logprob = torch.empty(lead, dtype=torch.float32, device=dev)
+        logprob = per_row()
         a.targets, a.logprob = targets.data_ptr(), logprob.data_ptr()
     logits, a.rows, a.seq, a.row_stride, a.batch_stride = _logit_rows(logits)
     a.logits, a.vocab, a.ignore_index, a.top = logits.data_ptr(), logits.shape[-1], ignore_index, top
-    stats = torch.empty((a.rows, 2), dtype=torch.float32, device=dev)
+    stats = torch.empty_strided((a.rows, 2), (2, 1), dtype=torch.float32, device=dev)
     a.stats = stats.data_ptr()
-    h = index = best = None
     if entropy:
-        h = torch.empty(lead, dtype=torch.float32, device=dev)
+        h = torch.empty_like(logprob) if logprob is not None else per_row()
         a.entropy = h.data_ptr()
     if top > 0:
-        index = torch.empty((*lead, top), dtype=torch.int64, device=dev)
-        best = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+        if flat:
+            index = torch.empty_strided((lead[0], top), (top, 1), dtype=torch.int64, device=dev)
+            best = torch.empty_strided((lead[0], top), (top, 1), dtype=torch.float32, device=dev)
+        else:
+            index = torch.empty((*lead, top), dtype=torch.int64, device=dev)
+            best = torch.empty((*lead, top), dtype=torch.float32, device=dev)
         a.top_index, a.top_logprob = index.data_ptr(), best.data_ptr()
-    with _on(dev):
-        check(lib.hyc_token_logprobs(C.byref(a), _stream(dev)), "hyc_token_logprobs")
+    _launch(lib.hyc_token_logprobs, "hyc_token_logprobs", a, device)
     return TokenLogprobs(logprob, h, index, best, stats)
 
 
@@ -284,13 +309,12 @@ def token_logprobs_bwd(logits: torch.Tensor, stats: torch.Tensor, targets: Optio
                        top_index: Optional[torch.Tensor] = None, d_top: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gradient with respect to ``logits`` (their dtype, contiguous) of what arrives for the results of
     :func:`token_logprobs`; ``stats``, ``entropy`` and ``top_index`` are those results.  Each of the three may be missing."""
-    _require_cuda(logits, stats, targets, d_logprob, entropy, d_entropy, top_index, d_top)
-    _same_device(logits, stats, targets, d_logprob, entropy, d_entropy, top_index, d_top)
+    device = _device_of(logits, stats, targets, d_logprob, entropy, d_entropy, top_index, d_top)
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise ValueError("logits must have a last dimension of at least one value")
     a = HycLogprobBwdArgs()
     a.dtype = _dtype_code(logits)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    grad = _result(logits)
     if d_logprob is not None:
         if targets is None:
             raise ValueError("a gradient of the log probabilities needs the targets")
@@ -317,6 +341,5 @@ def token_logprobs_bwd(logits: torch.Tensor, stats: torch.Tensor, targets: Optio
         _check_row_stats("d_top", d_top, rows * a.top)
         a.top_index, a.d_top = top_index.data_ptr(), d_top.data_ptr()
     a.logits, a.vocab, a.ignore_index, a.stats, a.grad = logits.data_ptr(), logits.shape[-1], ignore_index, stats.data_ptr(), grad.data_ptr()
-    with _on(grad.device):
-        check(lib.hyc_token_logprobs_bwd(C.byref(a), _stream(grad.device)), "hyc_token_logprobs_bwd")
+    _launch(lib.hyc_token_logprobs_bwd, "hyc_token_logprobs_bwd", a, device)
     return grad
