@@ -43,14 +43,15 @@ struct LnBwdArgs {
 //   VEC 1  16-byte pieces (8 bf16 or 4 fp32): thread t owns the pieces t, t + G, ...; every address of every row is 16-byte
 //          aligned and a row is a multiple of eight elements;
 //   VEC 2  the same where the row fills its threads' slots exactly: no bounds are left to test;
-//   VEC 0  the elements t, t + G, ... (coalesced accesses of single elements, for odd widths and unaligned tensors).
+//   VEC 0  single elements, for odd widths and unaligned tensors: a warp's chunks of 128 consecutive ones, four sweeps of its
+//          lanes each, a chunk per half slot.
 
 template <int VEC>
 __device__ __forceinline__ bool ln_in(int c, int cols) { return VEC == 2 || c < cols; }
 
 template <typename T, int G, int VEC>
 __device__ __forceinline__ int ln_col(int t, int v, int j) {
-  if (!VEC) return (v * 8 + j) * G + t;
+  if (!VEC) return ((2 * v + (j >> 2)) * G + (t & ~31)) * 4 + (j & 3) * 32 + (t & 31);
   return sizeof(T) == 2 ? (v * G + t) * 8 + j : ((2 * v + (j >> 2)) * G + t) * 4 + (j & 3);
 }
 
@@ -177,11 +178,22 @@ __device__ __forceinline__ void ln_table_get(const float* table, int t, int v, f
   }
 }
 
-// base + (kept ? x * scale : 0) of a slot; `first` is the index of the row's first element in the tensor
+// base + (kept ? x * scale : 0) of a slot; `first` is the index of the row's first element in the tensor.  VEC: a thread draws
+// the words of its own elements, whole counter blocks.  Else a chunk of 128 elements starts s = first % 4 elements into a
+// block: lane l draws the chunk's block l, ballots tell every lane all 128 keep bits, and the 33rd block, which the chunk's
+// last s elements are in, has been drawn for all chunks of the row at once (ln_ends: lane q holds its bits for chunk q).
+template <int G, int VPT, int VEC>
+__device__ __forceinline__ uint32_t ln_ends(Philox& gen, const DropRate& rate, unsigned long long first, int t) {
+  if (VEC || (first & 3) == 0) return 0;
+  const unsigned q = t & 31;
+  const uint4 w = gen.at(((first + (static_cast<unsigned>(q % (2 * VPT)) * G + (t & ~31)) * 4) >> 2) + 32);
+  return (rate.keep(w.x) ? 1u : 0u) | (rate.keep(w.y) ? 2u : 0u) | (rate.keep(w.z) ? 4u : 0u) | (rate.keep(w.w) ? 8u : 0u);
+}
+
 template <typename T, int G, int VEC, bool BASE>
-__device__ __forceinline__ void ln_drop(Philox& gen, const DropRate& rate, unsigned long long first, int t, int v, f32x2 (&x)[4],
-                                        const f32x2 (&base)[4]) {
-  uint32_t w[8];
+__device__ __forceinline__ void ln_drop(Philox& gen, const DropRate& rate, unsigned long long first, uint32_t ends, int t, int v,
+                                        f32x2 (&x)[4], const f32x2 (&base)[4]) {
+  bool keep[8];
   if (VEC) {                                   // rows of a multiple of eight elements: two whole counter blocks
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -191,15 +203,23 @@ __device__ __forceinline__ void ln_drop(Philox& gen, const DropRate& rate, unsig
         if (static_cast<uint32_t>(at >> 32) != gen.upper) gen.prepare(static_cast<uint32_t>(at >> 32));
       }
       const uint4 q = gen.block(static_cast<uint32_t>(at) + (sizeof(T) == 2 ? h : 0));
-      w[4 * h] = q.x; w[4 * h + 1] = q.y; w[4 * h + 2] = q.z; w[4 * h + 3] = q.w;
+      keep[4 * h] = rate.keep(q.x); keep[4 * h + 1] = rate.keep(q.y); keep[4 * h + 2] = rate.keep(q.z); keep[4 * h + 3] = rate.keep(q.w);
     }
   } else {
+    const int lane = t & 31, s = static_cast<int>(first & 3), word = (s + lane) & 3, block = (s + lane) >> 2;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const unsigned long long element = first + static_cast<unsigned>(ln_col<T, G, VEC>(t, v, j));
-      const uint4 q = gen.at(element >> 2);
-      const uint32_t lane = static_cast<uint32_t>(element & 3);
-      w[j] = lane == 0 ? q.x : lane == 1 ? q.y : lane == 2 ? q.z : q.w;
+    for (int h = 0; h < 2; ++h) {
+      const unsigned long long chunk = first + static_cast<unsigned>(ln_col<T, G, VEC>(t & ~31, v, 4 * h));
+      const uint4 q = gen.at((chunk >> 2) + lane);
+      const uint32_t b0 = __ballot_sync(0xffffffffu, rate.keep(q.x)), b1 = __ballot_sync(0xffffffffu, rate.keep(q.y));
+      const uint32_t b2 = __ballot_sync(0xffffffffu, rate.keep(q.z)), b3 = __ballot_sync(0xffffffffu, rate.keep(q.w));
+      const uint32_t bits = word == 0 ? b0 : word == 1 ? b1 : word == 2 ? b2 : b3;
+      const uint32_t end = __shfl_sync(0xffffffffu, ends, 2 * v + h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = 8 * j + block;                    // 0 .. 32
+        keep[4 * h + j] = j == 3 && at == 32 ? end >> word & 1 : bits >> (at & 31) & 1;
+      }
     }
   }
   if (rate.none) {
@@ -212,7 +232,7 @@ __device__ __forceinline__ void ln_drop(Philox& gen, const DropRate& rate, unsig
     float lo, hi, b0 = 0.f, b1 = 0.f;
     f2_split(BASE ? f2_fma(x[i], scale, base[i]) : f2_mul(x[i], scale), lo, hi);
     if (BASE) f2_split(base[i], b0, b1);
-    x[i] = f2_make(rate.keep(w[2 * i]) ? lo : b0, rate.keep(w[2 * i + 1]) ? hi : b1);
+    x[i] = f2_make(keep[2 * i] ? lo : b0, keep[2 * i + 1] ? hi : b1);
   }
 }
 
@@ -311,9 +331,12 @@ template <typename T, int G, int VPT, bool DROP, int VEC, bool TABLE>
 __device__ __forceinline__ void ln_fwd_row(const LnFwdArgs& a, Philox& gen, long long row, int t, f32x2 (&z)[VPT][4], f32x2 (&r)[VPT][4],
                                            float* slot, const float* table) {
   f32x2 s2 = f2_both(0.f);
+  const unsigned long long element = static_cast<unsigned long long>(row) * a.cols;
+  uint32_t ends = 0;
+  if (DROP) ends = ln_ends<G, VPT, VEC>(gen, a.rate, element, t);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    if (DROP) ln_drop<T, G, VEC, true>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, t, v, z[v], r[v]);
+    if (DROP) ln_drop<T, G, VEC, true>(gen, a.rate, element, ends, t, v, z[v], r[v]);
     else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[v][i] = f2_add(z[v][i], r[v][i]);
@@ -557,6 +580,8 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 || VPT > 2 ? 1 : 2
     f2_split(s1, b0, b1);
     const float2 s = group_sum2<G>(a0 + a1, b0 + b1, slots[group][turn]);
     const f32x2 minus_c2 = f2_both(-s.x * per_col), minus_c1 = f2_both(-s.y * per_col);
+    uint32_t ends = 0;
+    if (DROP) ends = ln_ends<G, VPT, VEC>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, t);
     void* out = static_cast<T*>(a.dresidual) + row * a.cols;
     void* dx = static_cast<T*>(a.dx) + row * a.cols;
 #pragma unroll
@@ -572,7 +597,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 || VPT > 2 ? 1 : 2
       }
       ln_put<T, G, VEC>(out, t, v, a.cols, d);
       if (DROP) {
-        ln_drop<T, G, VEC, false>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, t, v, d, d);
+        ln_drop<T, G, VEC, false>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, ends, t, v, d, d);
         ln_put<T, G, VEC>(dx, t, v, a.cols, d);
       }
     }
@@ -679,7 +704,7 @@ constexpr int ln_stages(int table, int most) {
 template <typename T, int G, int VPT, bool DROP, int VEC>
 static int run_ln_fwd(const LnFwdArgs& a, cudaStream_t stream) {
   constexpr int kThreads = G < 256 ? 256 : G, kGroups = kThreads / G, kTable = 2 * VPT * 8 * G * 4;
-  constexpr bool kHasTable = kTable <= 64 * 1024;
+  constexpr bool kHasTable = kTable + 2 * 2 * VPT * 8 * static_cast<int>(sizeof(T)) * kThreads <= (kThreads == 512 ? 220 : 110) * 1024;
   constexpr int kStages = VEC ? ln_stages<T, VPT, kThreads>(kHasTable ? kTable : 0, 2) : 0;
   if constexpr (kStages > 0) {
     if (a.rows >= 4LL * kGroups * sm_count()) {
@@ -715,6 +740,7 @@ static int pick_ln_fwd(const LnFwdArgs& a, bool vec, cudaStream_t stream) {
   if (slots <= 256) return pick_ln_fwd_kind<T, 128, 2>(a, vec, stream);
   if (slots <= 512) return pick_ln_fwd_kind<T, 256, 2>(a, vec, stream);
   if (slots <= 1024) return pick_ln_fwd_kind<T, 512, 2>(a, vec, stream);
+  if (slots <= 1536) return pick_ln_fwd_kind<T, 512, 3>(a, vec, stream);
   return pick_ln_fwd_kind<T, 512, 4>(a, vec, stream);
 }
 
@@ -770,6 +796,7 @@ static int pick_ln_bwd(const LnBwdArgs& a, bool vec, cudaStream_t stream) {
   if (slots <= 256) return pick_ln_bwd_kind<T, 128, 2, false>(a, vec, stream);
   if (slots <= 512) return pick_ln_bwd_kind<T, 256, 2, false>(a, vec, stream);
   if (slots <= 1024) return pick_ln_bwd_kind<T, 512, 2, false>(a, vec, stream);
+  if (slots <= 1536) return pick_ln_bwd_kind<T, 512, 3, true>(a, vec, stream);
   return pick_ln_bwd_kind<T, 512, 4, true>(a, vec, stream);
 }
 
