@@ -46,6 +46,12 @@ struct LnBwdArgs {
 //   VEC 0  single elements, for odd widths and unaligned tensors: a warp's chunks of 128 consecutive ones, four sweeps of its
 //          lanes each, a chunk per half slot.
 
+// single elements, by the read-only path: no store in between holds the loads back
+__device__ __forceinline__ float ln_one(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float ln_one(const __nv_bfloat16* p) {
+  return __uint_as_float(static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(p))) << 16);
+}
+
 template <int VEC>
 __device__ __forceinline__ bool ln_in(int c, int cols) { return VEC == 2 || c < cols; }
 
@@ -54,6 +60,12 @@ __device__ __forceinline__ int ln_col(int t, int v, int j) {
   if (!VEC) return ((2 * v + (j >> 2)) * G + (t & ~31)) * 4 + (j & 3) * 32 + (t & 31);
   return sizeof(T) == 2 ? (v * G + t) * 8 + j : ((2 * v + (j >> 2)) * G + t) * 4 + (j & 3);
 }
+
+// Single elements: whether any thread of the warp has one of the row in slot v; else the warp passes over it.  The backward pass
+// does so for the words alone: with branches around its loads 16384 x 1003 takes 94 us, not 82.  The forward pass gains by them
+// (8192 x 4099: 219 us, not 322).
+template <typename T, int G, int VEC>
+__device__ __forceinline__ bool ln_any(int t, int v, int cols) { return VEC != 0 || ln_col<T, G, VEC>(t & ~31, v, 0) < cols; }
 
 // a 16-byte piece as fp32 pairs, at f
 __device__ __forceinline__ void ln_unpack(const uint4& w, __nv_bfloat16, f32x2* f) {
@@ -69,8 +81,13 @@ __device__ __forceinline__ void ln_unpack(const uint4& w, float, f32x2* f) {
 __device__ __forceinline__ f32x2 f2_both(float v) { return f2_make(v, v); }
 
 // the eight elements of slot v of thread t as four pairs, zero beyond the row's end
-template <typename T, int G, int VEC>
+template <typename T, int G, int VEC, bool SKIP = false>
 __device__ __forceinline__ void ln_get(const void* row, int t, int v, int cols, f32x2 (&f)[4]) {
+  if (SKIP && !ln_any<T, G, VEC>(t, v, cols)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = 0;
+    return;
+  }
   if (VEC) {
     constexpr int kPiece = 16 / sizeof(T);
 #pragma unroll
@@ -83,15 +100,21 @@ __device__ __forceinline__ void ln_get(const void* row, int t, int v, int cols, 
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int c = ln_col<T, G, VEC>(t, v, j);
-      e[j] = c < cols ? static_cast<float>(static_cast<const T*>(row)[c]) : 0.f;
+      if (sizeof(T) == 2) {                   // 16-bit loads under a condition are branched around, one wait each: 103 us, not 68
+        const float one = ln_one(static_cast<const T*>(row) + min(c, cols - 1));
+        e[j] = c < cols ? one : 0.f;
+      } else {
+        e[j] = c < cols ? ln_one(static_cast<const T*>(row) + c) : 0.f;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = f2_make(e[2 * i], e[2 * i + 1]);
   }
 }
 
-template <typename T, int G, int VEC>
+template <typename T, int G, int VEC, bool SKIP = false>
 __device__ __forceinline__ void ln_put(void* row, int t, int v, int cols, const f32x2 (&p)[4]) {
+  if (SKIP && !ln_any<T, G, VEC>(t, v, cols)) return;
   float f[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) f2_split(p[i], f[2 * i], f[2 * i + 1]);
@@ -145,10 +168,16 @@ __device__ __forceinline__ void ln_param(const void* p, bool bf16, int t, int v,
   } else {
     float e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = ln_col<T, G, VEC>(t, v, j);
-      e[j] = fill;
-      if (c < cols) e[j] = bf16 ? static_cast<float>(static_cast<const __nv_bfloat16*>(p)[c]) : static_cast<const float*>(p)[c];
+    for (int j = 0; j < 8; ++j) e[j] = fill;                           // beyond the end: any finite value
+    if (bf16) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = ln_one(static_cast<const __nv_bfloat16*>(p) + min(ln_col<T, G, VEC>(t, v, j), cols - 1));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = ln_col<T, G, VEC>(t, v, j);
+        if (c < cols) e[j] = ln_one(static_cast<const float*>(p) + c);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = f2_make(e[2 * i], e[2 * i + 1]);
@@ -336,8 +365,9 @@ __device__ __forceinline__ void ln_fwd_row(const LnFwdArgs& a, Philox& gen, long
   if (DROP) ends = ln_ends<G, VPT, VEC>(gen, a.rate, element, t);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    if (DROP) ln_drop<T, G, VEC, true>(gen, a.rate, element, ends, t, v, z[v], r[v]);
-    else {
+    if (DROP) {
+      if (ln_any<T, G, VEC>(t, v, a.cols)) ln_drop<T, G, VEC, true>(gen, a.rate, element, ends, t, v, z[v], r[v]);
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[v][i] = f2_add(z[v][i], r[v][i]);
     }
@@ -371,7 +401,7 @@ __device__ __forceinline__ void ln_fwd_row(const LnFwdArgs& a, Philox& gen, long
   if (a.z) {
     void* zp = static_cast<T*>(a.z) + row * a.cols;
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) ln_put<T, G, VEC>(zp, t, v, a.cols, z[v]);
+    for (int v = 0; v < VPT; ++v) ln_put<T, G, VEC, true>(zp, t, v, a.cols, z[v]);
   }
   const f32x2 rstd2 = f2_both(rstd);
 #pragma unroll
@@ -386,7 +416,7 @@ __device__ __forceinline__ void ln_fwd_row(const LnFwdArgs& a, Philox& gen, long
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = f2_fma(f2_mul(f2_add(z[v][i], minus_mean), rstd2), w[i], b[i]);
-    ln_put<T, G, VEC>(y, t, v, a.cols, w);
+    ln_put<T, G, VEC, true>(y, t, v, a.cols, w);
   }
 }
 
@@ -439,7 +469,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 ? 1 : VPT <= 2 ? 3
 
 // One row per group (inputs of few rows, where a ring would only lengthen the way; rows without 16-byte alignment).
 template <typename T, int G, int VPT, bool DROP, int VEC>
-__global__ void __launch_bounds__(G < 256 ? 256 : G) ln_fwd_kernel(const LnFwdArgs a) {
+__global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 ? 1 : 3) ln_fwd_kernel(const LnFwdArgs a) {
   constexpr int kThreads = G < 256 ? 256 : G, kGroups = kThreads / G;
   __shared__ __align__(16) float slots[kGroups][64];
   const int t = group_thread<G, kGroups>(), group = group_index<G, kGroups>();
@@ -448,11 +478,11 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G) ln_fwd_kernel(const LnFwdAr
   const void* x = static_cast<const T*>(a.x) + row * a.x_stride;
   f32x2 z[VPT][4], r[VPT][4];
 #pragma unroll
-  for (int v = 0; v < VPT; ++v) ln_get<T, G, VEC>(x, t, v, a.cols, z[v]);
+  for (int v = 0; v < VPT; ++v) ln_get<T, G, VEC, true>(x, t, v, a.cols, z[v]);
   if (a.residual) {
     const void* res = static_cast<const T*>(a.residual) + row * a.residual_stride;
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) ln_get<T, G, VEC>(res, t, v, a.cols, r[v]);
+    for (int v = 0; v < VPT; ++v) ln_get<T, G, VEC, true>(res, t, v, a.cols, r[v]);
   } else {
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
@@ -596,13 +626,14 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 || VPT > 2 ? 1 : 2
         for (int i = 0; i < 4; ++i) d[i] = f2_add(d[i], e[i]);
       }
       ln_put<T, G, VEC>(out, t, v, a.cols, d);
-      if (DROP) {
+      if (DROP && ln_any<T, G, VEC>(t, v, a.cols)) {
         ln_drop<T, G, VEC, false>(gen, a.rate, static_cast<unsigned long long>(row) * a.cols, ends, t, v, d, d);
         ln_put<T, G, VEC>(dx, t, v, a.cols, d);
       }
     }
   }
   if (!a.partials) return;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   float* part = a.partials + static_cast<long long>(blockIdx.x) * 2 * a.cols;
   auto leave = [&](int c0, int c1, const ulonglong2& p) {
     float lo, hi;
@@ -641,25 +672,30 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 || VPT > 2 ? 1 : 2
   }
 }
 
-// The partial rows, summed in a fixed order: 32 columns per CTA, eight lanes of rows.
-__global__ void __launch_bounds__(256) ln_finish_kernel(const LnBwdArgs a) {
-  __shared__ float sums[8][33];
+// The partial rows, summed in a fixed order: 32 columns per CTA, 32 lanes of rows.  Launched while the kernel above runs out
+// (programmatic dependent launch): it waits for that one's partial rows before it reads them.
+__global__ void __launch_bounds__(1024) ln_finish_kernel(const LnBwdArgs a) {
+  __shared__ float sums[32][33];
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float s = 0.f;
   if (c < 2 * a.cols) {
 #pragma unroll 8
-    for (int part = lane; part < a.parts; part += 8) s += a.partials[static_cast<long long>(part) * 2 * a.cols + c];
+    for (int part = lane; part < a.parts; part += 32) s += a.partials[static_cast<long long>(part) * 2 * a.cols + c];
   }
   sums[lane][threadIdx.x & 31] = s;
   __syncthreads();
-  if (lane == 0 && c < 2 * a.cols) {
+  // warp w adds up column w: lane l holds partial sum l
+  const int col = blockIdx.x * 32 + lane;
+  float t = sums[threadIdx.x & 31][lane];
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sums[k][threadIdx.x & 31];
-    void* out = c < a.cols ? a.dweight : a.dbias;
-    const int at = c < a.cols ? c : c - a.cols;
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if ((threadIdx.x & 31) == 0 && col < 2 * a.cols) {
+    void* out = col < a.cols ? a.dweight : a.dbias;
+    const int at = col < a.cols ? col : col - a.cols;
     if (out) {
-      if (a.param_bf16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(s);
-      else static_cast<float*>(out)[at] = s;
+      if (a.param_bf16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(t);
+      else static_cast<float*>(out)[at] = t;
     }
   }
 }
@@ -739,6 +775,7 @@ static int pick_ln_fwd(const LnFwdArgs& a, bool vec, cudaStream_t stream) {
   if (slots <= 128) return pick_ln_fwd_kind<T, 32, 4>(a, vec, stream);
   if (slots <= 256) return pick_ln_fwd_kind<T, 128, 2>(a, vec, stream);
   if (slots <= 512) return pick_ln_fwd_kind<T, 256, 2>(a, vec, stream);
+  if (slots <= 768) return pick_ln_fwd_kind<T, 256, 3>(a, vec, stream);
   if (slots <= 1024) return pick_ln_fwd_kind<T, 512, 2>(a, vec, stream);
   if (slots <= 1536) return pick_ln_fwd_kind<T, 512, 3>(a, vec, stream);
   return pick_ln_fwd_kind<T, 512, 4>(a, vec, stream);
@@ -772,8 +809,14 @@ static int run_ln_bwd(LnBwdArgs a, cudaStream_t stream) {
   kernel<<<a.parts, kThreads, smem, stream>>>(a);
   HYC_LAUNCHED();
   if (a.partials) {
-    ln_finish_kernel<<<(2 * a.cols + 31) / 32, 256, 0, stream>>>(a);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((2 * a.cols + 31) / 32); cfg.blockDim = dim3(1024); cfg.stream = stream; cfg.attrs = &attr; cfg.numAttrs = 1;
+    const cudaError_t f = cudaLaunchKernelEx(&cfg, ln_finish_kernel, a);
     HYC_LAUNCHED();
+    if (f != cudaSuccess) return cuda_fail(f, "ln_finish_kernel");
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? HYC_OK : cuda_fail(e, "ln_bwd_kernel");
