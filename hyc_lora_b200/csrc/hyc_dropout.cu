@@ -50,11 +50,11 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs a) {
   }
 }
 
-// One flat run of elements at 16-byte aligned addresses.  Persistent: a CTA takes tiles of U * 256 pieces of 16 bytes and has
-// the next tile's loads in flight while it draws this tile's words.  Without a residual and in bf16 the generator's
-// multiplications (see hyc_philox.cuh) bound it next to DRAM, else DRAM alone.  Many words per turn keep the multiplier fed:
-// 8192 x 11008 bf16 takes 74 us with U = 8, 77 with 6, 80 with 4, 83 with 2 and 79 with 12 (DRAM alone: 56).
-
+// One flat run of elements at 16-byte aligned addresses.  Persistent: a CTA takes tiles of U * NT pieces of 16 bytes and has the
+// next tile's loads in flight while it draws this tile's words.  Without a residual and in bf16 the generator's products (see
+// hyc_philox.cuh) bound it, else DRAM.  Many words per thread keep the multiplier fed: 16384 x 11008 bf16 takes 141 us (DRAM
+// alone: 112; the products alone: 97) with U = 8 and 256 threads, 143 with 384, 160 with 512, and 83 / 74 of what U = 2 takes.
+// With a residual 384 threads of U = 4 take 67 us at 16384 x 4096 (DRAM: 62), 256 threads 75.
 // eight bf16 values as fp32; both halves by byte permutes and masks, which leave the multiplier's pipe to the generator
 __device__ __forceinline__ void piece_to_floats(const uint4& w, float (&f)[8]) {
   const uint32_t q[4] = {w.x, w.y, w.z, w.w};
@@ -72,7 +72,7 @@ __device__ __forceinline__ uint4 floats_to_piece(const float (&f)[4]) {
   return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
 }
 
-template <typename T, bool RES, int U>
+template <typename T, bool RES, int U, int NT>
 struct DropTile {
   static constexpr int kPiece = 16 / sizeof(T), kBlocks = kPiece / 4;
   uint4 x[U], r[U];
@@ -80,8 +80,8 @@ struct DropTile {
   __device__ __forceinline__ void load(const DropoutArgs& a, long long first) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      x[u] = load16_stream(static_cast<const uint4*>(a.x) + first + u * 256);
-      if (RES) r[u] = load16_stream(static_cast<const uint4*>(a.residual) + first + u * 256);
+      x[u] = load16_stream(static_cast<const uint4*>(a.x) + first + u * NT);
+      if (RES) r[u] = load16_stream(static_cast<const uint4*>(a.residual) + first + u * NT);
     }
   }
   __device__ __forceinline__ static uint4 piece(const DropoutArgs& a, const Philox& gen, const uint4& xp, const uint4& rp, uint32_t block) {
@@ -104,17 +104,21 @@ struct DropTile {
     const unsigned long long block = static_cast<unsigned long long>(first) * kBlocks;
     if (static_cast<uint32_t>(block >> 32) != gen.upper) gen.prepare(static_cast<uint32_t>(block >> 32));
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      static_cast<uint4*>(a.y)[first + u * 256] = piece(a, gen, x[u], r[u], static_cast<uint32_t>(block) + u * 256 * kBlocks);
+    for (int u = 0; u < U; ++u) {
+      const unsigned long long at = block + u * NT * kBlocks;
+      // tiles of a power of two never run across a change of the upper half
+      if ((U * NT & (U * NT - 1)) != 0 && static_cast<uint32_t>(at >> 32) != gen.upper) gen.prepare(static_cast<uint32_t>(at >> 32));
+      static_cast<uint4*>(a.y)[first + u * NT] = piece(a, gen, x[u], r[u], static_cast<uint32_t>(at));
+    }
   }
 };
 
-template <typename T, bool RES, int U>
-__global__ void __launch_bounds__(256, 1) dropout_flat_kernel(const DropoutArgs a) {
-  using Tile = DropTile<T, RES, U>;
-  constexpr int kTile = 256 * U, kBlocks = Tile::kBlocks;
+template <typename T, bool RES, int U, int NT>
+__global__ void __launch_bounds__(NT, 1) dropout_flat_kernel(const DropoutArgs a) {
+  using Tile = DropTile<T, RES, U, NT>;
+  constexpr int kTile = NT * U, kBlocks = Tile::kBlocks;
   Philox gen = Philox::load(a.rng);
-  const long long pieces = a.cols / Tile::kPiece, tiles = pieces / kTile;    // a tile's counters share their upper half
+  const long long pieces = a.cols / Tile::kPiece, tiles = pieces / kTile;
   if (!a.rate.none) {
     Tile one, two;
     long long tile = blockIdx.x;
@@ -131,12 +135,12 @@ __global__ void __launch_bounds__(256, 1) dropout_flat_kernel(const DropoutArgs 
       tile = next;
     }
   } else {
-    for (long long p = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; p < tiles * kTile; p += static_cast<long long>(gridDim.x) * 256)
+    for (long long p = static_cast<long long>(blockIdx.x) * NT + threadIdx.x; p < tiles * kTile; p += static_cast<long long>(gridDim.x) * NT)
       static_cast<uint4*>(a.y)[p] = RES ? static_cast<const uint4*>(a.residual)[p] : make_uint4(0, 0, 0, 0);
   }
   // the pieces behind the last whole tile, and the elements behind the last piece
   if (blockIdx.x != tiles % gridDim.x) return;
-  for (long long p = tiles * kTile + threadIdx.x; p < pieces; p += 256) {
+  for (long long p = tiles * kTile + threadIdx.x; p < pieces; p += NT) {
     const unsigned long long block = static_cast<unsigned long long>(p) * kBlocks;
     if (static_cast<uint32_t>(block >> 32) != gen.upper) gen.prepare(static_cast<uint32_t>(block >> 32));
     const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -159,13 +163,13 @@ __global__ void rng_take_kernel(unsigned long long* state, long long* used) {
   used[1] = static_cast<long long>(atomicAdd(state + 1, 1ull));
 }
 
-template <typename T, bool RES, int U>
+template <typename T, bool RES, int U, int NT>
 static void run_dropout_flat(const DropoutArgs& a, cudaStream_t stream) {
-  auto kernel = dropout_flat_kernel<T, RES, U>;
-  const long long blocks = a.cols / (256 * U * (16 / sizeof(T))) + 1;
+  auto kernel = dropout_flat_kernel<T, RES, U, NT>;
+  const long long blocks = a.cols / (NT * U * (16 / sizeof(T))) + 1;
   static PerDevice resident;
-  const long long most = resident.get([&] { return resident_grid(kernel, 256, 0, 1 << 20); });
-  kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(a);
+  const long long most = resident.get([&] { return resident_grid(kernel, NT, 0, 1 << 20); });
+  kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), NT, 0, stream>>>(a);
 }
 
 template <typename T>
@@ -175,11 +179,11 @@ static int launch_dropout(const DropoutArgs& a, cudaStream_t stream) {
     // small tensors: one piece per thread on as many SMs as there are
     const bool large = a.cols * static_cast<long long>(sizeof(T)) >= 16LL * 256 * 8 * 4 * sm_count();
     if (a.residual) {
-      if (large) run_dropout_flat<T, true, 4>(a, stream);
-      else run_dropout_flat<T, true, 1>(a, stream);
+      if (large) run_dropout_flat<T, true, 4, 384>(a, stream);
+      else run_dropout_flat<T, true, 1, 256>(a, stream);
     } else {
-      if (large) run_dropout_flat<T, false, 8>(a, stream);
-      else run_dropout_flat<T, false, 1>(a, stream);
+      if (large) run_dropout_flat<T, false, 8, 256>(a, stream);
+      else run_dropout_flat<T, false, 1, 256>(a, stream);
     }
   } else {
     const long long blocks = (a.rows * a.cols + 1023) / 1024;

@@ -134,6 +134,22 @@ def test_dropout_beyond_32_bit_offsets(ops):
     _near(ops.dropout(rows, 0.25, _rng().cuda()), *ro.dropout(rows.cpu(), 0.25, ro.keep_mask(11, 5, 0.25, (3, 512))))
 
 
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_dropout_where_the_counter_passes_32_bits(ops, with_residual):
+    """Element 2^34 begins counter block 2^32."""
+    n = 2 ** 34 + 100003
+    x = torch.ones(n, dtype=BF16, device="cuda")
+    y = ops.dropout(x, 0.25, _rng().cuda(), residual=x if with_residual else None)
+    for first in (0, 2 ** 33, 2 ** 34 - 20000, 2 ** 34 - 64, 2 ** 34 + 64, n - 128):
+        count = 40000 if first == 2 ** 34 - 20000 else 128
+        keep = ro.keep_mask(11, 5, 0.25, (count,), first=first)
+        one = torch.ones(count, dtype=BF16)
+        want, bound = ro.dropout(one, 0.25, keep, one if with_residual else None)
+        _near(y[first:first + count], want, bound, str(first))
+    del x, y
+    torch.cuda.empty_cache()
+
+
 def test_generator_calls_and_replayed_graphs(ops):
     state = _rng(9, 0).cuda()
     taken = [ops.rng_take(state).tolist() for _ in range(3)]
