@@ -231,6 +231,10 @@ int hyc_dropout(const hyc_dropout_args* args, void* stream) {
   a.rows = args->rows; a.cols = args->cols; a.x_stride = args->x_stride; a.residual_stride = args->residual_stride;
   a.rng = reinterpret_cast<const long long*>(args->rng);
   a.rate = DropRate::make(args->p);
+  if (a.x_stride == a.cols && (!a.residual || a.residual_stride == a.cols)) {      // rows without gaps: one flat run
+    a.cols *= a.rows;
+    a.rows = 1;
+  }
   return args->dtype == HYC_BF16 ? launch_dropout<__nv_bfloat16>(a, static_cast<cudaStream_t>(stream))
                                  : launch_dropout<float>(a, static_cast<cudaStream_t>(stream));
 }
