@@ -77,8 +77,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 //      m, and the values of the pieces that hold it are tested for it.  At the row's end the warps' sums are joined.
 //   2. alternatives: every thread also knows the largest value it has seen.  The k-th largest of 64 groups' maxima is a bound
 //      that the k best reach and hardly anything else does; the few threads that have seen something that reaches it have
-//      their pieces read again (from L2) by the whole CTA, what reaches the bound is collected, and each counts those before
-//      it.  Where too many reach it (rows of equal values, or hardly anything open), or the row holds a NaN, the best are
+//      their pieces read again (from L2) by their warp, what reaches the bound is collected, and each counts those before it.  Where too many reach it (rows of equal values, or hardly anything open), or the row holds a NaN, the best are
 //      picked one after the other instead.
 // Few long rows are split over the CTAs of a cluster, which work on slices with their own m; the first one joins sums and
 // alternatives through distributed shared memory, in rank order: no atomics on results, no workspace, one launch.
@@ -292,9 +291,7 @@ __device__ __noinline__ void lp_pick_slowly(const LpRow r, int vocab, int top, u
 struct LpShared {
   LpSums part[2][8];                       // [parity][warp]
   float4 group[kLpGroups / 4];
-  float bound;
-  int hot, found;
-  unsigned short hots[256];                // threads that have seen something that reaches the bound
+  int found;
   unsigned long long keys[kLpCandidates];
   unsigned long long picked[32];
   unsigned long long best[8];
@@ -517,6 +514,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS > 24 ? 24 : 768 / THREA
     }
     if (kWarps > 1 || TOP) {
       if (lane == 0) sh.part[turn][warp] = s;
+      if (TOP && threadIdx.x == 0) sh.found = 0;         // the last row's has been read by everybody, a barrier ago
       __syncthreads();
     }
     if (warp == 0) {
@@ -532,55 +530,54 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS > 24 ? 24 : 768 / THREA
     }
     // 2. the alternatives
     if (TOP) {
-      // The bound: the group maximum that top - 1 others stand before.  kPerGroup threads per group, each counting in its
-      // share of the others.
-      {
-        const int g = threadIdx.x / kPerGroup, p = threadIdx.x % kPerGroup;
-        constexpr int kShare = kGroups / 4 / kPerGroup;
-        const float v = reinterpret_cast<const float*>(sh.group)[g];
-        int before = 0;
-#pragma unroll 4
-        for (int q = 0; q < kShare; ++q) {
-          const int j = p * kShare + q;
-          const float4 o = sh.group[j];
-          before += (o.x > v || (o.x == v && 4 * j < g)) + (o.y > v || (o.y == v && 4 * j + 1 < g)) +
-                    (o.z > v || (o.z == v && 4 * j + 2 < g)) + (o.w > v || (o.w == v && 4 * j + 3 < g));
-        }
-#pragma unroll
-        for (int o = 1; o < kPerGroup; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-        if (p == 0 && before == a.top - 1) sh.bound = v;
-        if (threadIdx.x == 0) sh.hot = sh.found = 0;
-      }
-      __syncthreads();
-      const float bound = sh.bound;
-      if (mine >= bound) sh.hots[atomicAdd(&sh.hot, 1)] = static_cast<unsigned short>(threadIdx.x);
-      // a NaN anywhere in the slice: in a group's maximum, so in the first thread's count of them; its own test is cheaper
-      bool nan = false;
-      if (threadIdx.x < kGroups) nan = reinterpret_cast<const float*>(sh.group)[threadIdx.x] != reinterpret_cast<const float*>(sh.group)[threadIdx.x];
-      const bool slow_nan = __syncthreads_or(nan);
+      bool slow_nan;
       const LpRow r = lp_row<T>(a.logits, lp_offset(a, row), a.vocab, rank, ranks);
-      const int hot = sh.hot, sweeps = r.pieces > 0 ? (r.pieces + THREADS - 1) / THREADS : 0;
-      for (int k = threadIdx.x; k < hot * sweeps && !slow_nan; k += THREADS) {
-        const int piece = sh.hots[k % hot] + (k / hot) * THREADS;
-        if (piece >= r.pieces) continue;
-        const uint4 w = lp_fetch<T>(r, a.vocab, piece);
-        if (!(lp_piece_max<T>(w) >= bound)) continue;
-        float f[kPiece];
-        lp_unpack<T>(w, f);
-        uint32_t reach = 0;
-#pragma unroll
-        for (int e = 0; e < kPiece; ++e) reach |= f[e] >= bound ? 1u << e : 0u;
-        const int e0 = (r.first + piece) * kPiece - r.lead;
-        while (reach) {                                        // hardly ever more than one
-          const int e = __ffs(reach) - 1;
-          reach &= reach - 1;
-          if (e0 + e < 0 || e0 + e >= a.vocab) continue;
-          const int word = sizeof(T) == 2 ? e >> 1 : e;
-          const uint32_t bits = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
-          const float x = __uint_as_float(sizeof(T) == 4 ? bits : e & 1 ? bits & 0xffff0000u : bits << 16);
-          const int at = atomicAdd(&sh.found, 1);
-          if (at < kLpCandidates) sh.keys[at] = lp_key(x, e0 + e);
+      // The bound, by every warp for itself: the largest group maximum, taken away top - 1 times.
+      float g0 = reinterpret_cast<const float*>(sh.group)[lane], g1 = -INFINITY;
+      if (kGroups > 32) g1 = reinterpret_cast<const float*>(sh.group)[lane + 32];
+      slow_nan = __any_sync(0xffffffffu, g0 != g0 || g1 != g1);
+      float bound = lp_warp_max(lp_max(g0, g1));
+      for (int k = 1; k < a.top && bound != -INFINITY && !slow_nan; ++k) {
+        const uint32_t b0 = __ballot_sync(0xffffffffu, g0 == bound), b1 = __ballot_sync(0xffffffffu, g1 == bound);
+        if (b0) {
+          if (lane == __ffs(b0) - 1) g0 = -INFINITY;
+        } else if (lane == __ffs(b1) - 1) {
+          g1 = -INFINITY;
         }
+        bound = lp_warp_max(lp_max(g0, g1));
+      }
+      // a warp's threads that have seen something that reaches it: their pieces again, two threads' at a time
+      uint32_t hot = slow_nan ? 0u : __ballot_sync(0xffffffffu, mine >= bound);
+      const int sweeps = r.pieces > 0 ? (r.pieces + THREADS - 1) / THREADS : 0;
+      while (hot) {
+        const int h0 = __ffs(hot) - 1;
+        hot &= hot - 1;
+        const int h1 = hot ? __ffs(hot) - 1 : -1;
+        hot &= hot - 1;                                          // of 0: 0
+        const int h = lane < 16 ? h0 : h1;
+        for (int k = h >= 0 ? lane & 15 : sweeps; k < sweeps; k += 16) {
+          const int piece = warp * 32 + h + k * THREADS;
+          if (piece >= r.pieces) continue;
+          const uint4 w = lp_fetch<T>(r, a.vocab, piece);
+          if (!(lp_piece_max<T>(w) >= bound)) continue;
+          float f[kPiece];
+          lp_unpack<T>(w, f);
+          uint32_t reach = 0;
+#pragma unroll
+          for (int e = 0; e < kPiece; ++e) reach |= f[e] >= bound ? 1u << e : 0u;
+          const int e0 = (r.first + piece) * kPiece - r.lead;
+          while (reach) {                                        // hardly ever more than one
+            const int e = __ffs(reach) - 1;
+            reach &= reach - 1;
+            if (e0 + e < 0 || e0 + e >= a.vocab) continue;
+            const int word = sizeof(T) == 2 ? e >> 1 : e;
+            const uint32_t bits = word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w;
+            const float x = __uint_as_float(sizeof(T) == 4 ? bits : e & 1 ? bits & 0xffff0000u : bits << 16);
+            const int at = atomicAdd(&sh.found, 1);
+            if (at < kLpCandidates) sh.keys[at] = lp_key(x, e0 + e);
+          }
+        }
+        __syncwarp();
       }
       __syncthreads();
       const int found = sh.found;
@@ -662,7 +659,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS > 24 ? 24 : 768 / THREA
 // Elementwise over the logits with five numbers per row: a CTA (or, for short rows, a warp) takes a run of pieces of one row,
 // kLpPieces per thread.  What arrives for single tokens is put right afterwards by the threads that hold those few, after a
 // barrier that orders their stores behind the run's.
-constexpr int kLpPieces = 4;
+constexpr int kLpWarpPieces = 4, kLpPieces = 8;
 
 template <typename T>
 __device__ __forceinline__ void lp_store_piece(void* p, const float (&f)[16 / sizeof(T)]);
@@ -754,9 +751,9 @@ struct LpGrad {
 // A warp takes a whole short row (WARP), a CTA one run of kWidth * kLpPieces pieces of a longer one.
 template <typename T, bool WARP, bool ENT>
 __global__ void __launch_bounds__(256) logprob_bwd_kernel(const LogprobBwdArgs a) {
-  constexpr int kPiece = 16 / sizeof(T), kWidth = WARP ? 32 : 256;
+  constexpr int kPiece = 16 / sizeof(T), kWidth = WARP ? 32 : 256, kPer = WARP ? kLpWarpPieces : kLpPieces;
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int row = WARP ? static_cast<int>(blockIdx.x * 8 + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x), run = WARP ? 0 : blockIdx.y;
+    const int row = WARP ? static_cast<int>(blockIdx.x * 8 + (threadIdx.x >> 5)) : static_cast<int>(blockIdx.x), run = WARP ? 0 : blockIdx.y;
   if (WARP && (row >= a.rows || row < 0)) return;
   const T* x = static_cast<const T*>(a.logits) + lp_offset(a, row);
   T* out = static_cast<T*>(a.grad) + static_cast<long long>(row) * a.vocab;
@@ -765,16 +762,16 @@ __global__ void __launch_bounds__(256) logprob_bwd_kernel(const LogprobBwdArgs a
   // pieces counted from the aligned address at or below the row's start, if x and out lie alike
   const int phase = static_cast<int>(reinterpret_cast<uintptr_t>(out) & 15u), lead = phase / static_cast<int>(sizeof(T));
   const bool alike = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15u) == phase;
-  const int first = run * (kWidth * kLpPieces), last = min((lead + a.vocab + kPiece - 1) / kPiece, first + kWidth * kLpPieces);
+  const int first = run * (kWidth * kPer), last = min((lead + a.vocab + kPiece - 1) / kPiece, first + kWidth * kPer);
   g.ready(a);
-  uint4 raw[kLpPieces];
+  uint4 raw[kPer];
 #pragma unroll
-  for (int i = 0; i < kLpPieces; ++i) {
+  for (int i = 0; i < kPer; ++i) {
     const int piece = first + i * kWidth + t, e0 = piece * kPiece - lead;
     if (piece < last && alike && !g.zero && e0 >= 0 && e0 + kPiece <= a.vocab) raw[i] = load16_stream(x + e0);
   }
 #pragma unroll
-  for (int i = 0; i < kLpPieces; ++i) {
+  for (int i = 0; i < kPer; ++i) {
     const int piece = first + i * kWidth + t, e0 = piece * kPiece - lead;
     if (piece >= last) continue;
     if (alike && e0 >= 0 && e0 + kPiece <= a.vocab) {
@@ -914,8 +911,8 @@ static void run_logprob_bwd(const LogprobBwdArgs& a, int runs, cudaStream_t stre
 template <typename T>
 static int launch_logprob_bwd(const LogprobBwdArgs& a, cudaStream_t stream) {
   const long long pieces = (static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1;
-  const bool warp = pieces <= 32 * kLpPieces;                       // short rows: a warp each
-  const int width = (warp ? 32 : 256) * kLpPieces, runs = static_cast<int>((pieces + width - 1) / width);
+  const bool warp = pieces <= 32 * kLpWarpPieces;                       // short rows: a warp each
+  const int width = warp ? 32 * kLpWarpPieces : 256 * kLpPieces, runs = static_cast<int>((pieces + width - 1) / width);
   if (warp) a.d_entropy ? run_logprob_bwd<T, true, true>(a, runs, stream) : run_logprob_bwd<T, true, false>(a, runs, stream);
   else a.d_entropy ? run_logprob_bwd<T, false, true>(a, runs, stream) : run_logprob_bwd<T, false, false>(a, runs, stream);
   HYC_LAUNCHED();
