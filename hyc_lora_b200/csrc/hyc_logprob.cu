@@ -77,8 +77,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 //      m, and the values of the pieces that hold it are tested for it.  At the row's end the warps' sums are joined.
 //   2. alternatives: every thread also knows the largest value it has seen.  The k-th largest of 64 groups' maxima is a bound
 //      that the k best reach and hardly anything else does; the few threads that have seen something that reaches it have
-//      their pieces read again (from L2) by their warp, what reaches the bound is collected, and each counts those before it.  Where too many reach it (rows of equal values, or hardly anything open), or the row holds a NaN, the best are
-//      picked one after the other instead.
+//      their pieces read again (from L2) by their warp, what reaches the bound is collected, and each counts those before it.
+//      Where too many reach it (equal values; fewer open tokens than alternatives), what stands above the bound is collected
+//      and the first of its equals in index order with it; where the row holds a NaN, the best are picked one after the other.
 // Few long rows are split over the CTAs of a cluster, which work on slices with their own m; the first one joins sums and
 // alternatives through distributed shared memory, in rank order: no atomics on results, no workspace, one launch.
 //
@@ -290,6 +291,7 @@ __device__ __noinline__ void lp_pick_slowly(const LpRow r, int vocab, int top, u
 
 struct LpShared {
   LpSums part[2][8];                       // [parity][warp]
+  int ties[8];                             // [warp]
   float4 group[kLpGroups / 4];
   int found;
   unsigned long long keys[kLpCandidates];
@@ -299,6 +301,61 @@ struct LpShared {
   LpSums slice[2][8];                      // [parity][rank], in the first CTA of a cluster
   unsigned long long slice_keys[2][8][32];
 };
+
+// Candidates of a row in which very many equal the bound: all that is above it, and as many of its equals, lowest index first,
+// as are still wanted.  Returns how many there are (more than kLpCandidates: too many above).  All threads of the CTA.
+template <typename T, int THREADS>
+__device__ __noinline__ int lp_collect_ties(const LpRow r, int vocab, int top, float bound, LpShared* sh) {
+  constexpr int kPiece = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();
+  if (threadIdx.x == 0) sh->found = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < r.pieces; i += THREADS) {
+    const uint4 w = lp_fetch<T>(r, vocab, i);
+    if (!(lp_piece_max<T>(w) > bound)) continue;
+    float f[kPiece];
+    lp_unpack<T>(w, f);
+    const int e0 = (r.first + i) * kPiece - r.lead;
+#pragma unroll
+    for (int e = 0; e < kPiece; ++e) {
+      if (!(f[e] > bound)) continue;                               // beyond the row: -inf, above nothing
+      const int at = atomicAdd(&sh->found, 1);
+      if (at < kLpCandidates) sh->keys[at] = lp_key(f[e], e0 + e);
+    }
+  }
+  __syncthreads();
+  int wanted = top - sh->found;
+  if (wanted > 0 && sh->found + wanted > kLpCandidates) return kLpCandidates + 1;
+  for (int first = 0; first < r.pieces && wanted > 0; first += THREADS) {
+    const int i = first + threadIdx.x;
+    const uint4 w = lp_fetch<T>(r, vocab, i);
+    float f[kPiece];
+    lp_unpack<T>(w, f);
+    const int e0 = (r.first + i) * kPiece - r.lead;
+    uint32_t equal = 0;
+#pragma unroll
+    for (int e = 0; e < kPiece; ++e) equal |= i < r.pieces && f[e] == bound && e0 + e >= 0 && e0 + e < vocab ? 1u << e : 0u;
+    int before = __popc(equal);                                    // inclusive over the lanes, then over the warps
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int lower = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += lower;
+    }
+    if (lane == 31) sh->ties[warp] = before;
+    before -= __popc(equal);
+    __syncthreads();
+    int all = 0;
+    for (int v = 0; v < THREADS / 32; ++v) {
+      if (v == warp) before += all;
+      all += sh->ties[v];
+    }
+    for (; equal && before < wanted; equal &= equal - 1, ++before) sh->keys[atomicAdd(&sh->found, 1)] = lp_key(bound, e0 + __ffs(equal) - 1);
+    wanted -= all;
+    __syncthreads();
+  }
+  return sh->found;
+}
 
 // sums of up to eight parts, one per lane; complete in the first eight lanes
 __device__ __forceinline__ LpSums lp_join(LpSums s, bool have) {
@@ -547,9 +604,11 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS > 24 ? 24 : 768 / THREA
         bound = lp_warp_max(lp_max(g0, g1));
       }
       // a warp's threads that have seen something that reaches it: their pieces again, two threads' at a time
-      uint32_t hot = slow_nan ? 0u : __ballot_sync(0xffffffffu, mine >= bound);
+      uint32_t hot = slow_nan || bound == -INFINITY ? 0u : __ballot_sync(0xffffffffu, mine >= bound);
       const int sweeps = r.pieces > 0 ? (r.pieces + THREADS - 1) / THREADS : 0;
       while (hot) {
+        // more than can be kept: equal values, see below
+        if (__shfl_sync(0xffffffffu, *const_cast<volatile int*>(&sh.found), 0) > kLpCandidates) break;
         const int h0 = __ffs(hot) - 1;
         hot &= hot - 1;
         const int h1 = hot ? __ffs(hot) - 1 : -1;
@@ -580,7 +639,8 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS > 24 ? 24 : 768 / THREA
         __syncwarp();
       }
       __syncthreads();
-      const int found = sh.found;
+      int found = sh.found;
+      if (found > kLpCandidates || (bound == -INFINITY && !slow_nan)) found = lp_collect_ties<T, THREADS>(r, a.vocab, a.top, bound, &sh);
       auto put = [&](int place, unsigned long long key) {
         if (!CLUSTER) {
           sh.picked[place] = key;

@@ -498,6 +498,29 @@ def test_logprobs_of_rows_without_a_choice(ops, dtype, vocab):
     _check_grads(ops, x, x.cuda(), out, t, 4)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,vocab", [(5, 700), (3, 32000), (300, 4100), (3, 100003)])
+def test_logprobs_alternatives_among_very_many_equal_values(ops, dtype, rows, vocab):
+    """Rows whose k-th best value is shared by more elements than are collected: a few open tokens among masked ones, two levels,
+    equal values that begin late in the row."""
+    low = torch.finfo(dtype).min
+    x = torch.full((rows, vocab), -INF, dtype=dtype)
+    x[0, [vocab - 1, 3, vocab // 2]] = torch.tensor([1.0, 5.0, 5.0], dtype=dtype)
+    x[1] = low
+    x[1, vocab // 3:vocab // 3 + 7] = _randn((7,), dtype, 1)
+    x[2, : vocab // 2] = -3.0
+    x[2, vocab // 2:] = 2.0
+    x[2, -1] = 4.0
+    for row in range(3, rows):
+        x[row] = low if row % 2 else -INF
+        open_ = torch.randperm(vocab, generator=_gen(row))[: row % 25]
+        x[row, open_] = _randn((len(open_),), dtype, row)
+    t = torch.arange(rows) % vocab
+    for top in (1, 4, 20, 32):
+        _check_logprobs(ops, x, t, x.cuda(), top)
+    _check_logprobs(ops, x, t, _offset(x, 1), 20)
+
+
 def test_logprobs_with_nan_and_infinity(ops):
     x, t = _logit_inputs(5, 3001, F32, 3)
     t[1] = 7
