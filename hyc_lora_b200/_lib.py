@@ -160,13 +160,14 @@ SYMBOLS = {
     "hyc_nf4_dequant": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     "hyc_rope": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                            C.c_int32, C.c_void_p]),
+    # the row operators' records are passed by address: a ctypes record by reference, or its bytes (rowops packs them)
     "hyc_rng_take": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
-    "hyc_dropout": (C.c_int, [C.POINTER(HycDropoutArgs), C.c_void_p]),
-    "hyc_layer_norm": (C.c_int, [C.POINTER(HycLayerNormArgs), C.c_void_p]),
+    "hyc_dropout": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "hyc_layer_norm": (C.c_int, [C.c_void_p, C.c_void_p]),
     "hyc_layer_norm_bwd_scratch_floats": (C.c_int64, [C.c_int64, C.c_int32]),
-    "hyc_layer_norm_bwd": (C.c_int, [C.POINTER(HycLayerNormBwdArgs), C.c_void_p]),
-    "hyc_token_logprobs": (C.c_int, [C.POINTER(HycLogprobArgs), C.c_void_p]),
-    "hyc_token_logprobs_bwd": (C.c_int, [C.POINTER(HycLogprobBwdArgs), C.c_void_p]),
+    "hyc_layer_norm_bwd": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "hyc_token_logprobs": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "hyc_token_logprobs_bwd": (C.c_int, [C.c_void_p, C.c_void_p]),
     "hyc_select_channels_static_max_cols": (C.c_int, []),
     "hyc_select_channels_noalloc": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
 }

@@ -1,8 +1,8 @@
 """Token log probabilities with entropy and alternatives, and the language-model loss made of them.
 
-The host models of the reference take their loss from an fp32 copy of the shifted logits (models/modeling_llama.py, the
-``CrossEntropyLoss`` at the end of the forward pass); here the logits are read in their own dtype, two floats per row are kept,
-and the gradient is written once in the logits' dtype."""
+The host models take their loss by eager ops from an fp32 copy of the shifted logits (reference: models/modeling_llama.py);
+here the logits are read in their own dtype, two floats per row are kept, and the gradient is written once in the logits'
+dtype."""
 import torch
 
 from .. import rowops

@@ -160,6 +160,16 @@ def test_logprob_refusals(lib):
 
 # ------------------------------------------------------------------------------------------------ refusals in Python
 
+def test_packed_records_have_the_layout_of_the_ctypes_ones(lib):
+    from hyc_lora_b200 import rowops
+    codes = {C.c_int64: "q", C.c_int32: "i", C.c_void_p: "P", C.c_float: "f", C.c_double: "d"}
+    for packer, record in ((rowops._DROPOUT, lib.HycDropoutArgs), (rowops._LAYER_NORM, lib.HycLayerNormArgs),
+                           (rowops._LAYER_NORM_BWD, lib.HycLayerNormBwdArgs), (rowops._LOGPROB, lib.HycLogprobArgs),
+                           (rowops._LOGPROB_BWD, lib.HycLogprobBwdArgs)):
+        assert packer.format == "@" + "".join(codes[kind] for _, kind in record._fields_)
+        assert packer.size == C.sizeof(record)
+
+
 def test_python_refuses_cpu_tensors_and_wrong_arguments(lib):
     from hyc_lora_b200 import rowops
     x, rng = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64)
