@@ -78,6 +78,17 @@ __device__ __forceinline__ void ln_unpack(const uint4& w, float, f32x2* f) {
   f[0] = f2_make(__uint_as_float(w.x), __uint_as_float(w.y));
   f[1] = f2_make(__uint_as_float(w.z), __uint_as_float(w.w));
 }
+// A packed add takes both halves of the fp32 pipe, one of which also multiplies integers; two single ones can keep to the other.
+// Beside the generator that is worth the issue slots in the rows of several warps (65536 x 4096 backward with dropout: 468 us,
+// not 486), in those of one warp it is not (65536 x 768: 84 us, not 82.5).
+template <bool APART>
+__device__ __forceinline__ f32x2 ln_add(f32x2 a, f32x2 b) {
+  if (!APART) return f2_add(a, b);
+  float a0, a1, b0, b1;
+  f2_split(a, a0, a1);
+  f2_split(b, b0, b1);
+  return f2_make(a0 + b0, a1 + b1);
+}
 __device__ __forceinline__ f32x2 f2_both(float v) { return f2_make(v, v); }
 
 // the eight elements of slot v of thread t as four pairs, zero beyond the row's end
@@ -498,7 +509,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 ? 1 : 3) ln_fwd_ke
 
 // Where the parameter gradients of a thread's own columns add up over its rows: registers, or (rows so wide that they would
 // not fit beside the row) shared memory, one conflict-free column of it per thread.  Pairs of columns.
-template <int VPT, bool SMEM, int THREADS>
+template <int VPT, bool SMEM, int THREADS, bool APART>
 struct LnAcc {
   f32x2 w[VPT][4], b[VPT][4];
   __device__ __forceinline__ void init(void*) {
@@ -509,12 +520,12 @@ struct LnAcc {
   }
   __device__ __forceinline__ void add(int v, int i, f32x2 dy, f32x2 u) {
     w[v][i] = f2_fma(dy, u, w[v][i]);
-    b[v][i] = f2_add(dy, b[v][i]);
+    b[v][i] = ln_add<APART>(dy, b[v][i]);
   }
   __device__ __forceinline__ ulonglong2 get(int v, int i) const { return make_ulonglong2(w[v][i], b[v][i]); }
 };
-template <int VPT, int THREADS>
-struct LnAcc<VPT, true, THREADS> {
+template <int VPT, int THREADS, bool APART>
+struct LnAcc<VPT, true, THREADS, APART> {
   ulonglong2* own;
   __device__ __forceinline__ void init(void* smem) {
     own = static_cast<ulonglong2*>(smem) + threadIdx.x;
@@ -538,7 +549,8 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 || VPT > 2 ? 1 : 2
   extern __shared__ __align__(16) unsigned char staged[];
   __shared__ __align__(16) float slots[kGroups][2][32];
   const int t = group_thread<G, kGroups>(), group = group_index<G, kGroups>();
-  LnAcc<VPT, SMEM, kThreads> acc;
+  constexpr bool kApart = DROP && G > 32;
+  LnAcc<VPT, SMEM, kThreads, kApart> acc;
   acc.init(staged);
   Philox gen = {};
   if (DROP) gen = Philox::load(a.rng);
@@ -598,10 +610,10 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 || VPT > 2 ? 1 : 2
       else ln_param<T, G, VEC>(a.weight, a.param_bf16, t, v, a.cols, 1.f, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u[v][i] = f2_mul(f2_add(u[v][i], minus_mean), rstd2);
+        u[v][i] = f2_mul(ln_add<kApart>(u[v][i], minus_mean), rstd2);
         acc.add(v, i, g[v][i], u[v][i]);
         g[v][i] = f2_mul(g[v][i], w[i]);
-        s0 = f2_add(s0, g[v][i]);
+        s0 = ln_add<kApart>(s0, g[v][i]);
         s1 = f2_fma(g[v][i], u[v][i], s1);
       }
     }
@@ -618,7 +630,7 @@ __global__ void __launch_bounds__(G < 256 ? 256 : G, G == 512 || VPT > 2 ? 1 : 2
     for (int v = 0; v < VPT; ++v) {
       f32x2 d[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = f2_mul(f2_fma(u[v][i], minus_c1, f2_add(g[v][i], minus_c2)), rstd2);
+      for (int i = 0; i < 4; ++i) d[i] = f2_mul(f2_fma(u[v][i], minus_c1, ln_add<kApart>(g[v][i], minus_c2)), rstd2);
       if (a.dz) {
         f32x2 e[4];
         ln_get<T, G, VEC>(static_cast<const T*>(a.dz) + row * a.dz_stride, t, v, a.cols, e);

@@ -1,5 +1,6 @@
 """The row operators on the GPU against their plain 64-bit forms (oracle/rowops_oracle.py), whose bounds count roundings."""
 import copy
+import os
 
 import pytest
 import torch
@@ -9,6 +10,7 @@ from oracle import rowops_oracle as ro
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
 INF = float("inf")
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -521,14 +523,19 @@ def test_logprobs_alternatives_among_very_many_equal_values(ops, dtype, rows, vo
     _check_logprobs(ops, x, t, _offset(x, 1), 20)
 
 
-def test_logprobs_with_nan_and_infinity(ops):
-    x, t = _logit_inputs(5, 3001, F32, 3)
+@pytest.mark.parametrize("vocab", [300, 3001, 40000, 100001])
+def test_logprobs_with_nan_and_infinity(ops, vocab):
+    """Short rows, rows of one CTA and rows that are spread over a cluster, of which one slice holds the NaN."""
+    x, t = _logit_inputs(5, vocab, F32, 3)
     t[1] = 7
-    x[1, 100], x[2, 5] = float("nan"), INF
+    x[1, vocab // 3], x[2, 5] = float("nan"), INF
     out = ops.token_logprobs(x.cuda(), t.cuda(), entropy=True, top=3)
     for row in (1, 2):
         assert out.logprob[row].isnan() and out.entropy[row].isnan() and bool(out.top_logprob[row].isnan().all())
-    assert out.top_index[1, 0].item() == 100 and out.top_index[2, 0].item() == 5
+    assert out.top_index[1, 0].item() == vocab // 3 and out.top_index[2, 0].item() == 5
+    finite = x[1].clone()
+    finite[vocab // 3] = -INF
+    assert out.top_index[1, 1].item() == finite.argmax().item()
     rest = torch.tensor([0, 3, 4])
     want, bound = ro.token_logprobs(x[rest], t[rest], top=3)
     _near(out.logprob[rest.cuda()], want["logprob"], bound["logprob"])
@@ -839,6 +846,35 @@ class _WithLabels(torch.nn.Module):
 
     def forward(self, ids):
         return self.model(ids, self.labels)
+
+
+def test_first_calls_inside_a_capture():
+    """A fresh process whose very first call of each operator is recorded into a graph."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from hyc_lora_b200 import rowops as o
+x = torch.randn(2500, 4096, device='cuda', dtype=torch.bfloat16)
+w, lg, t = torch.ones(4096, device='cuda'), torch.randn(8, 70000, device='cuda'), torch.zeros(8, dtype=torch.int64, device='cuda')
+state = torch.tensor([1, 0], device='cuda')
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    rng = o.rng_take(state)
+    out = o.layer_norm(o.dropout(x, 0.1, rng, residual=x), w, w, residual=x, p=0.1, rng=rng)
+    back = o.layer_norm_bwd(x, out.z, w, out.mean, out.rstd, p=0.1, rng=rng)
+    lp = o.token_logprobs(lg, t, entropy=True, top=5)
+    grad = o.token_logprobs_bwd(lg, lp.stats, t, lp.logprob)
+g.replay()
+torch.cuda.synchronize()
+rng = torch.tensor([1, 0], device='cuda')
+again = o.layer_norm(o.dropout(x, 0.1, rng, residual=x), w, w, residual=x, p=0.1, rng=rng)
+assert torch.equal(again.y, out.y) and state.tolist() == [1, 1]
+assert torch.equal(o.token_logprobs(lg, t, entropy=True, top=5).entropy, lp.entropy)
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_tensors_of_two_devices_are_refused(ops):
