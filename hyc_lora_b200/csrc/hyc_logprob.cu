@@ -85,8 +85,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 //
 // Issue slots are as scarce as bytes here: bf16 leaves 11 of them per 32 elements at full bandwidth, and the exponentials take
 // 8 of their unit's cycles.  Holding whole rows in registers instead, with a barrier behind the maximum and one behind the
-// sums, took 122 us at 8192 x 32000 (512 threads of 8 pieces) or 186 (256 of 16), staging them in shared memory 151; this takes 104.
-// Chunks of 2 pieces take 107, of 6 113; two buffers that change places instead of a copy 114 (spills).
+// sums, took 122 us at 8192 x 32000 (512 threads of 8 pieces) or 186 (256 of 16), staging them in shared memory 151; this takes 104
+// with 256 threads per row and 91 with 64 (see lp_threads).  With 256, chunks of 2 pieces take 107, of 6 113; two buffers that
+// change places instead of a copy 114 (spills).
 constexpr int kLpCandidates = 256, kLpGroups = 64, kLpChunk = 4;
 
 struct alignas(16) LpSums {        // stored by 16 bytes into another CTA's shared memory
@@ -948,18 +949,49 @@ static int pick_logprob(const LogprobArgs& a, int ranks, cudaStream_t stream) {
   return a.entropy ? run_logprob<T, THREADS, true, false, CLUSTER>(a, ranks, stream) : run_logprob<T, THREADS, false, false, CLUSTER>(a, ranks, stream);
 }
 
-// Short rows: smaller CTAs, at least two chunks for each.  Few long rows are spread over clusters, as far as a slice keeps two
-// chunks and the SMs' places for CTAs go.
+// What `rows` rows take on CTAs of which the device holds `places` at once, relative to their bytes: whole rounds, a last one
+// that is not full but takes a third of a round at least, and what `extra` percent a row costs on such CTAs beside its bytes.
+static double lp_cost(long long rows, long long places, int extra) {
+  const long long whole = rows / places, rest = rows % places;
+  const double rounds = static_cast<double>(whole) + (rest ? 0.35 + 0.65 * static_cast<double>(rest) / static_cast<double>(places) : 0.0);
+  return rounds * static_cast<double>(places) * (100 + extra);
+}
+
+// Threads per row.  A row's end (joining the sums, finding the alternatives) is a chain of latencies that only other CTAs of
+// the SM fill, so small CTAs -- more of them, each with more of a row per thread -- do better; large ones do where there are too
+// few rows for all places, or where they leave a fuller last round.  Measured, us, with 256 / 128 / 64 threads (bf16, 32000
+// tokens): with five alternatives and entropy 8192 rows 146 / 128 / 130, 4096 rows 76 / 66 / 74, 1000 rows 25 / 21 / 23, 300
+// rows 10 / 12 / 16; log probabilities only 8192 rows 105 / 96 / 91, 4096 rows 56 / 50 / 52, 300 rows 9 / 10 / 12; fp32, 1024
+// rows of 50265 with entropy 41 / 44 / 39.  The percentages below are these, less the rounds.  Rows of fewer than two chunks
+// take fewer threads in any case.
+template <typename T>
+static int lp_threads(const LogprobArgs& a, long long pieces) {
+  if (pieces <= 2 * 32 * kLpChunk) return 32;
+  if (pieces > 2 * 128 * kLpChunk && a.rows <= sm_count() * 3) return 256;          // every row has a place of its own
+  const int most = pieces <= 2 * 64 * kLpChunk ? 64 : pieces <= 2 * 128 * kLpChunk ? 128 : 256;
+  int best = 64;
+  double least = lp_cost(a.rows, sm_count() * 12, a.top ? 55 : 9);
+  if (most >= 128) {
+    const double cost = lp_cost(a.rows, sm_count() * 6, a.top ? 53 : 16);
+    if (cost < least) { best = 128; least = cost; }
+  }
+  if (most >= 256 && lp_cost(a.rows, sm_count() * 3, a.top ? 78 : 28) < least) best = 256;
+  return best;
+}
+
+// Few long rows are spread over clusters, as far as a slice keeps two chunks and the SMs' places for CTAs go.
 template <typename T>
 static int launch_logprob(const LogprobArgs& a, cudaStream_t stream) {
   const long long pieces = (static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1;
   int ranks = 1;
   while (ranks < 8 && static_cast<long long>(a.rows) * ranks * 2 <= sm_count() * 4 && pieces / (ranks * 2) >= 512) ranks *= 2;
   if (ranks > 1) return pick_logprob<T, 256, true>(a, ranks, stream);
-  if (pieces <= 2 * 32 * kLpChunk) return pick_logprob<T, 32, false>(a, 1, stream);
-  if (pieces <= 2 * 64 * kLpChunk) return pick_logprob<T, 64, false>(a, 1, stream);
-  if (pieces <= 2 * 128 * kLpChunk) return pick_logprob<T, 128, false>(a, 1, stream);
-  return pick_logprob<T, 256, false>(a, 1, stream);
+  switch (lp_threads<T>(a, pieces)) {
+    case 32: return pick_logprob<T, 32, false>(a, 1, stream);
+    case 64: return pick_logprob<T, 64, false>(a, 1, stream);
+    case 128: return pick_logprob<T, 128, false>(a, 1, stream);
+    default: return pick_logprob<T, 256, false>(a, 1, stream);
+  }
 }
 
 template <typename T, bool WARP, bool ENT>
