@@ -218,7 +218,7 @@ struct LpSweep {
 };
 
 // Sums of one piece in base 2: with L = log2 e in fp32 and c = -m L rounded, u = x L + c in one rounding, e = 2^u; what c lost
-// to its rounding is a common factor that the row's sums are given at the end (lp_rescale).  APART: values equal to m are
+// to its rounding is a common factor that the sums are given at the end (lp_lost).  APART: values equal to m are
 // counted instead.
 template <typename T, bool ENT, bool APART>
 __device__ __forceinline__ void lp_piece_sums(const uint4& w, float m, f32x2 c, f32x2& rest, f32x2& te, float& count) {
@@ -248,13 +248,31 @@ __device__ __forceinline__ void lp_piece_sums(const uint4& w, float m, f32x2 c, 
   }
 }
 
-// sum of e and of e u -> sum of e and of e (x - m)
-__device__ __forceinline__ void lp_rescale(float m, float c, float& rest, float& te) {
-  const float lost = fmaf(-m, kLog2e, -c);             // exact
-  const float factor = exp2f(lost);
-  te = (te + lost * rest) * factor * 0.6931471805599453f;
-  rest *= factor;
+// The same for an m so far from zero that c would lose too much: from the differences themselves, c = 0.
+template <typename T>
+__device__ __forceinline__ void lp_piece_sums_far(const uint4& w, float m, f32x2& rest, f32x2& te, float& count) {
+  constexpr int kPiece = 16 / sizeof(T);
+  float f[kPiece], r = 0.f, t = 0.f;
+  lp_unpack<T>(w, f);
+#pragma unroll 1
+  for (int i = 0; i < kPiece; ++i) {
+    float x = f[0];
+#pragma unroll
+    for (int e = 1; e < kPiece; ++e) x = e == i ? f[e] : x;
+    if (x == m) {
+      count += 1.f;
+    } else {
+      const float u = lp_max((x - m) * kLog2e, -10000.f), e = lp_exp2(u);
+      r += e;
+      t = fmaf(e, u, t);
+    }
+  }
+  rest = f2_add(rest, f2_make(r, 0.f));
+  te = f2_add(te, f2_make(t, 0.f));
 }
+
+// what c = -m L has lost to its rounding: exact
+__device__ __forceinline__ float lp_lost(float m, float c, bool far) { return far ? 0.f : fmaf(-m, kLog2e, -c); }
 
 // the best `top` of this CTA's slice one after the other, from memory (rare: see above); keys in descending order to `out`
 template <typename T>
@@ -428,7 +446,7 @@ template <typename T, bool ENT>
 struct LpRunning {
   float m, c, count;             // m and c = -m log2(e) of the warp
   f32x2 rest, te;
-  bool far;                      // |m| so large that its neighbours in fp32 are 10^22 apart: e is 0 for all but m (and c may overflow)
+  bool far;                      // |m| of 2^20 or more, where c would lose over a tenth to its rounding
 
   __device__ __forceinline__ void clear() {
     m = -INFINITY;
@@ -436,45 +454,55 @@ struct LpRunning {
     rest = te = 0;
     far = true;
   }
+  // the sums so far, taken to a larger m: out of the old frame (what c lost, what equalled m), down by the difference, into the new
+  __device__ __forceinline__ void raise(float largest) {
+    const float old_m = m, lost = lp_lost(m, c, far);
+    m = lp_max(m, largest);
+    far = !(fabsf(m) < 1048576.f);
+    c = far ? 0.f : -m * kLog2e;
+    float r0, r1, t0, t1;
+    f2_split(rest, r0, r1);
+    f2_split(te, t0, t1);
+    const float down = (old_m - m) * kLog2e;
+    if (old_m == -INFINITY || !(down > -300.f)) {
+      r0 = r1 = t0 = t1 = 0.f;
+    } else {
+      const float out = lp_exp2(lost), f = lp_exp2(down), now = lp_lost(m, c, far), in = lp_exp2(-now);
+      t0 = (t0 + lost * r0) * out;
+      t1 = (t1 + lost * r1) * out;
+      r0 = r0 * out + count;
+      r1 *= out;
+      t0 = f * (t0 + down * r0);
+      t1 = f * (t1 + down * r1);
+      r0 *= f;
+      r1 *= f;
+      t0 = in * (t0 - now * r0);
+      t1 = in * (t1 - now * r1);
+      r0 *= in;
+      r1 *= in;
+    }
+    rest = f2_make(r0, r1);
+    te = f2_make(t0, t1);
+    count = 0.f;
+  }
   // a chunk, the thread's largest value of each piece and the warp's of all
   __device__ __forceinline__ void add(const uint4 (&w)[kLpChunk], const float (&most)[kLpChunk], float largest) {
-    if (!(largest < m)) {
-      if (largest != m) {        // what there is, to the new m
-        const bool was_far = far;
-        const float old = c;
-        m = lp_max(m, largest);
-        far = fabsf(m) >= 1e30f;
-        c = far ? 0.f : -m * kLog2e;
-        if (was_far || far) {
-          rest = te = 0;
-        } else {
-          float lo, hi;
-          const float up = c - old, f = lp_exp2(up);
-          f2_split(rest, lo, hi);
-          const f32x2 all = f2_make(lo + count, hi), f2 = f2_make(f, f);
-          if (ENT) te = f2_mul(f2, f2_fma(f2_make(up, up), all, te));
-          rest = f2_mul(f2, all);
-        }
-        count = 0.f;
+    const bool above = !(largest < m);                   // or a NaN
+    if (above && largest != m) raise(largest);
+    if (far) {
+      if (m == -INFINITY) return;                        // nothing open yet
+#pragma unroll
+      for (int i = 0; i < kLpChunk; ++i) lp_piece_sums_far<T>(w[i], m, rest, te, count);
+      return;
+    }
+    const f32x2 c2 = f2_make(c, c);
+    if (above) {
+#pragma unroll
+      for (int i = 0; i < kLpChunk; ++i) {
+        if (__any_sync(0xffffffffu, !(most[i] < m))) lp_piece_sums<T, ENT, true>(w[i], m, c2, rest, te, count);
+        else lp_piece_sums<T, ENT, false>(w[i], m, c2, rest, te, count);
       }
-      const f32x2 c2 = f2_make(c, c);
-      if (far) {
-#pragma unroll
-        for (int i = 0; i < kLpChunk; ++i) {
-          float f[16 / sizeof(T)];
-          lp_unpack<T>(w[i], f);
-#pragma unroll
-          for (int e = 0; e < static_cast<int>(16 / sizeof(T)); ++e) count += f[e] == m && m != -INFINITY ? 1.f : 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kLpChunk; ++i) {
-          if (__any_sync(0xffffffffu, !(most[i] < m))) lp_piece_sums<T, ENT, true>(w[i], m, c2, rest, te, count);
-          else lp_piece_sums<T, ENT, false>(w[i], m, c2, rest, te, count);
-        }
-      }
-    } else if (!far) {
-      const f32x2 c2 = f2_make(c, c);
+    } else {
 #pragma unroll
       for (int i = 0; i < kLpChunk; ++i) lp_piece_sums<T, ENT, false>(w[i], m, c2, rest, te, count);
     }
@@ -492,7 +520,9 @@ struct LpRunning {
       s.rest += __shfl_xor_sync(0xffffffffu, s.rest, o);
       if (ENT) s.te += __shfl_xor_sync(0xffffffffu, s.te, o);
     }
-    if (!far) lp_rescale(m, c, s.rest, s.te);
+    const float lost = lp_lost(m, c, far), out = exp2f(lost);
+    s.te = (s.te + lost * s.rest) * out * 0.6931471805599453f;
+    s.rest *= out;
     return s;
   }
 };

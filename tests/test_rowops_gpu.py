@@ -544,6 +544,18 @@ def test_logprobs_with_nan_and_infinity(ops, vocab):
     assert bool(g[1].isnan().all()) and bool(g[2].isnan().all()) and not bool(g[rest.cuda()].isnan().any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shift", [1000.0, -30000.0, 1.04e6, -1.2e6, 3e9, 1e20, -1e29, 1e31, -1e36])
+@pytest.mark.parametrize("rows,vocab", [(6, 1000), (6, 33000), (700, 2100)])
+def test_logprobs_of_logits_far_from_zero(ops, dtype, shift, rows, vocab):
+    """The differences are what counts: neither the size of the logits nor their sign costs digits."""
+    x, t = _logit_inputs(rows, vocab, F32, 9)
+    x = (x + shift).to(dtype)
+    out = _check_logprobs(ops, x, t, x.cuda(), 5)
+    if rows < 100:
+        _check_grads(ops, x, x.cuda(), out, t, 5)
+
+
 def test_logprobs_targets_outside_and_ignored(ops):
     x, t = _logit_inputs(6, 1000, BF16, 3)
     t[0], t[1], t[2], t[3] = -100, 1000, -1, 2 ** 40
