@@ -53,8 +53,9 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs a) {
 // One flat run of elements at 16-byte aligned addresses.  Persistent: a CTA takes tiles of U * NT pieces of 16 bytes and has the
 // next tile's loads in flight while it draws this tile's words.  Without a residual and in bf16 the generator's products (see
 // hyc_philox.cuh) bound it, else DRAM.  Many words per thread keep the multiplier fed: 16384 x 11008 bf16 takes 141 us (DRAM
-// alone: 112; the products alone: 97) with U = 8 and 256 threads, 143 with 384, 160 with 512, and 83 / 74 of what U = 2 takes.
-// With a residual 384 threads of U = 4 take 67 us at 16384 x 4096 (DRAM: 62), 256 threads 75.
+// alone: 112; the products alone: 97) with U = 8 and 256 threads, 143 with 384, 160 with 512; at 8192 x 11008 U = 8 takes 74 us,
+// U = 4 80, U = 2 83.  With a residual 384 threads of U = 4 take 69 us at 16384 x 4096 (DRAM: 62), 256 threads 75.
+
 // eight bf16 values as fp32; both halves by byte permutes and masks, which leave the multiplier's pipe to the generator
 __device__ __forceinline__ void piece_to_floats(const uint4& w, float (&f)[8]) {
   const uint32_t q[4] = {w.x, w.y, w.z, w.w};
@@ -176,8 +177,9 @@ template <typename T>
 static int launch_dropout(const DropoutArgs& a, cudaStream_t stream) {
   const bool flat = a.rows == 1 && aligned16(a.x) && aligned16(a.y) && aligned16(a.residual);
   if (flat) {
-    // small tensors: one piece per thread on as many SMs as there are
-    const bool large = a.cols * static_cast<long long>(sizeof(T)) >= 16LL * 256 * 8 * 4 * sm_count();
+    // One piece per thread, on as many SMs as there are, for small tensors.  Measured, us, one piece / many per thread: fp32 of
+    // 6 MB 4.2 / 6.4; bf16 of 18 MB 12.4 / 10.3, of 36 MB 22.3 / 18.5; with a residual of 18 MB 12.4 / 13.5, of 36 MB 24.8 / 22.9.
+    const bool large = a.cols * static_cast<long long>(sizeof(T)) >= 16LL * 256 * 8 * (a.residual ? 4 : 2) * sm_count();
     if (a.residual) {
       if (large) run_dropout_flat<T, true, 4, 384>(a, stream);
       else run_dropout_flat<T, true, 1, 256>(a, stream);
