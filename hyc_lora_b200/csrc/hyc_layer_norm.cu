@@ -331,6 +331,7 @@ __device__ __forceinline__ void group_sync() {
 // aligned) and is not used again before the group has met at another barrier.
 template <int G>
 __device__ __forceinline__ float group_sum(float v, float* slot) {
+  static_assert(G == 32 || G % 128 == 0, "warps are read four at a time");
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (G == 32) return v;
@@ -347,6 +348,7 @@ __device__ __forceinline__ float group_sum(float v, float* slot) {
 // two at once: after the first exchange each half of a warp carries one of them
 template <int G>
 __device__ __forceinline__ float2 group_sum2(float v0, float v1, float* slot) {
+  static_assert(G == 32 || G % 64 == 0, "warps are read two at a time");
   const bool upper = threadIdx.x & 16;
   float v = (upper ? v1 : v0) + __shfl_xor_sync(0xffffffffu, upper ? v0 : v1, 16);
 #pragma unroll
@@ -849,7 +851,11 @@ static int pick_ln_bwd(const LnBwdArgs& a, bool vec, cudaStream_t stream) {
   if (slots <= 32) return pick_ln_bwd_kind<T, 32, 1, false>(a, vec, stream);
   if (slots <= 64) return pick_ln_bwd_kind<T, 32, 2, false>(a, vec, stream);
   if (slots <= 96) return pick_ln_bwd_kind<T, 32, 3, false>(a, vec, stream);
-  if (slots <= 128) return pick_ln_bwd_kind<T, 128, 1, false>(a, vec, stream);
+  if (slots <= 128) {
+    // bf16: two warps of two slots (65536 x 1024 with dropout 106 us, 127 as four of one); fp32 the other way round (81 / 99)
+    if constexpr (sizeof(T) == 2) return pick_ln_bwd_kind<T, 64, 2, false>(a, vec, stream);
+    else return pick_ln_bwd_kind<T, 128, 1, false>(a, vec, stream);
+  }
   if (slots <= 256) return pick_ln_bwd_kind<T, 128, 2, false>(a, vec, stream);
   if (slots <= 512) return pick_ln_bwd_kind<T, 256, 2, false>(a, vec, stream);
   if (slots <= 1024) return pick_ln_bwd_kind<T, 512, 2, false>(a, vec, stream);
