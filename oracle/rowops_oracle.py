@@ -9,6 +9,9 @@ import torch
 
 U = 2.0 ** -24
 SLACK = 1.05
+# fp32's smallest normal number: an exponential below it may be taken as zero.  Where it enters by itself that is TINY at most,
+# where it is multiplied by a logarithm 100 * TINY (the logarithm of TINY is -87.3).
+TINY = 2.0 ** -126
 
 
 def half_step(dtype) -> float:
@@ -129,10 +132,10 @@ def token_logprobs(logits, targets, ignore_index=-100, top=0):
     finite_d = torch.where(e > 0, d, torch.zeros_like(d))
     others = torch.where(first, torch.zeros_like(e), e)
     drest = (others * _rel_exp(finite_d)).sum(1) + chain * U * rest
-    dlogz = drest / total + 3 * U * logz.abs()
+    dlogz = drest / total + 3 * U * logz.abs() + vocab * TINY
     entropy = torch.where(none, torch.zeros_like(rest), logz - ed.sum(1) / total)
     ted = ed.abs().sum(1)
-    dentropy = dlogz + ((ed.abs() * (_rel_exp(finite_d) + 2 * U)).sum(1) + chain * U * ted) / total + ted / total * (drest / total + 4 * U)
+    dentropy = dlogz + ((ed.abs() * (_rel_exp(finite_d) + 2 * U)).sum(1) + chain * U * ted) / total + ted / total * (drest / total + 4 * U) + 100 * vocab * TINY
     out, bound = {}, {}
 
     def logp_at(index):
@@ -188,6 +191,5 @@ def token_logprobs_bwd(logits, stats, targets=None, d_logprob=None, ignore_index
                                     torch.zeros_like(p)) + 2 * U * (grad.abs() + part.abs())
     grad = torch.where(none, torch.zeros_like(grad), grad)
     bound = torch.where(none, torch.zeros_like(bound), bound)
-    # below the type's smallest normal number a value may be flushed to zero
-    tiny = torch.finfo(torch.float32).tiny
-    return grad, SLACK * (bound + half_step(kind) * grad.abs()) + 2 * tiny * (1 + size + (d_entropy.double().abs()[:, None] if d_entropy is not None else 0))
+    flushed = 1 + size + (100 * d_entropy.double().abs()[:, None] if d_entropy is not None else 0)
+    return grad, SLACK * (bound + half_step(kind) * grad.abs()) + 2 * TINY * flushed
