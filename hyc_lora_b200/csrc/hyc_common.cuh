@@ -140,19 +140,13 @@ __device__ __forceinline__ void load8<float>(const float* row, int col, float (&
   f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
-// The same from global memory, for data that is read once: it does not displace what L1 holds.
+// 16 bytes of global memory that are read once: they do not displace what L1 holds.
 __device__ __forceinline__ uint4 load16_stream(const void* p) {
   uint4 w;
   asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                : "l"(p));
   return w;
-}
-__device__ __forceinline__ void load8_stream(const __nv_bfloat16* p, float (&f)[8]) { unpack_bf16x8(load16_stream(p), f); }
-__device__ __forceinline__ void load8_stream(const float* p, float (&f)[8]) {
-  const uint4 a = load16_stream(p), b = load16_stream(p + 4);
-  f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
-  f[4] = __uint_as_float(b.x); f[5] = __uint_as_float(b.y); f[6] = __uint_as_float(b.z); f[7] = __uint_as_float(b.w);
 }
 
 // fp32 tables of D entries that every thread reads 8 consecutive channels at a time (norm weights,
