@@ -434,6 +434,9 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// the two halves of a barrier that passes no data on
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // address of `p` (this CTA's shared memory) in the shared memory of CTA 0 of the cluster
 __device__ __forceinline__ uint32_t in_first_cta(const void* p) {
   uint32_t r;
@@ -532,6 +535,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS > 24 ? 24 : 768 / THREA
   constexpr int kPiece = 16 / sizeof(T), kWarps = THREADS / 32;
   constexpr int kPerGroup = THREADS <= kLpGroups ? 1 : THREADS / kLpGroups, kGroups = THREADS / kPerGroup;   // lanes of a group: 1, 2 or 4
   __shared__ LpShared sh;
+  if (CLUSTER) cluster_arrive();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0, ranks = CLUSTER ? static_cast<int>(cluster_size()) : 1;
   const int step = static_cast<int>(gridDim.x) / ranks;
@@ -555,6 +559,12 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS > 24 ? 24 : 768 / THREA
   if (row < a.rows) {
     sweep.start(a.logits, lp_offset(a, row), a.vocab, rank, ranks);
     sweep.load(0, a.vocab, cur);
+  }
+  if (CLUSTER) {
+    // The first CTA's shared memory may be written once that CTA is known to have started.  The wait passes under the first
+    // loads, and CTAs without a row take part.
+    __syncwarp();
+    cluster_wait();
   }
   int turn = 0;
   while (row < a.rows) {

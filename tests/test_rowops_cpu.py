@@ -1,12 +1,17 @@
 """No-GPU checks of the row operators: the generator against its published vectors, refusals at the C entry points and in
 Python, and the plain 64-bit forms the GPU tests compare with against torch's own."""
 import ctypes as C
+import glob
+import os
+import re
 
 import numpy as np
 import pytest
 import torch
 
 from oracle import rowops_oracle as ro
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hyc_lora_b200", "csrc")
 
 
 @pytest.fixture(scope="module")
@@ -233,3 +238,34 @@ def test_hosts_build_with_and_without_the_row_operators(lib):
         assert a == b and torch.equal(p, q)          # the same weights from the same seed
     ids, labels = torch.randint(0, 50, (2, 7)), torch.tensor([0, 1])
     assert torch.isfinite(plain(ids, labels))
+
+
+# ------------------------------------------------------------------------------------------------ orderings, read from the source
+
+def _kernel_bodies(text):
+    """(name, body) of every __global__ function of a source file."""
+    for found in re.finditer(r"__global__ void\s+(?:__launch_bounds__\((?:[^()]|\([^()]*\))*\)\s*)?(\w+)\(", text):
+        at = text.index("{", found.end())
+        depth, end = 1, at + 1
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+        yield found.group(1), text[at:end]
+
+
+def test_ctas_of_a_cluster_meet_before_they_write_into_one_another():
+    """Another CTA's shared memory may be accessed only after it is known to have started: a wait at a cluster barrier stands
+    in front of the first store, and one behind the last in front of the exit."""
+    seen = 0
+    for path in sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))):
+        text = open(path).read()
+        for name, body in _kernel_bodies(text):
+            stores = [m.start() for m in re.finditer(r"\b(?:ld|st|red|atom)\.(?:\w+\.)*shared::cluster\.", body)]
+            if not stores:
+                continue
+            seen += 1
+            waits = [m.start() for m in re.finditer(r"\bcluster_(?:wait|barrier)\(\)", body)]
+            assert waits and waits[0] < stores[0] and waits[-1] > stores[-1], (path, name)
+            if body[waits[0]:].startswith("cluster_wait"):
+                assert 0 <= body.find("cluster_arrive()") < waits[0], (path, name)
+    assert seen >= 1

@@ -661,6 +661,24 @@ def test_logprobs_row_counts(ops, rows, vocab):
     _near(ops.token_logprobs_bwd(x.cuda(), plain.stats, t.cuda(), d.cuda()), *ro.token_logprobs_bwd(x, out.stats.cpu(), t, d))
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 262144), (2, 32000), (40, 16385), (96, 70001), (130, 33000)])
+def test_logprobs_of_clusters_that_find_little_to_do(ops, rows, vocab):
+    """Rows spread over CTAs that meet at their start: all of them ignored (nothing is read), every other one, only the last."""
+    x, t = _logit_inputs(rows, vocab, BF16, rows)
+    xd = x.cuda()
+    for ignored in (torch.ones(rows, dtype=torch.bool), torch.arange(rows) % 2 == 0, torch.arange(rows) < rows - 1):
+        tt = torch.where(ignored, -100, t)
+        got = ops.token_logprobs(xd, tt.cuda())
+        want, bound = ro.token_logprobs(x, tt)
+        _near(got.logprob, want["logprob"], bound["logprob"])
+        assert bool((got.stats.cpu()[ignored] == torch.tensor([-INF, 0.0])).all())
+        _near(got.stats[~ignored.cuda()], want["stats"][~ignored], bound["stats"][~ignored])
+        again = ops.token_logprobs(xd, tt.cuda(), entropy=True, top=7)
+        want, bound = ro.token_logprobs(x, tt, top=7)
+        assert torch.equal(again.top_index.cpu(), want["top_index"])
+        _near(again.entropy, want["entropy"], bound["entropy"])
+
+
 def test_logprob_gradient_with_repeated_and_foreign_alternatives(ops):
     """An index that repeats, equals the target, or lies outside the vocabulary (which takes part in the sum only)."""
     x, t = _logit_inputs(4, 500, F32, 3)
