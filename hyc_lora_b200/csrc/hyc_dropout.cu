@@ -1,6 +1,9 @@
 // Dropout with the mask drawn from a counter (hyc_philox.cuh), with or without the add of a residual:
 //     y = residual + (keep ? x / (1 - p) : 0)
-// computed in fp32 and rounded once.  What is dropped is selected away, not multiplied by zero: an infinity or a NaN in a
+// The kept value x * scale, scale = 1 / (1 - p) in fp32, is rounded to fp32 before it is added: that rounding takes back what
+// the rounding of scale brought in wherever x / (1 - p) has few digits (x = 9 k, p = 0.1).  Fused, scale's error went on into
+// the sum: exact zeros came out as 1e-8 and ties of the output's rounding fell to one side.  The sum is rounded to fp32 and
+// then once to the output's type.  What is dropped is selected away, not multiplied by zero: an infinity or a NaN in a
 // dropped place does not reach y.  The backward pass is the same kernel on the arriving gradient.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -26,6 +29,13 @@ __device__ __forceinline__ float to_float<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// product and sum each rounded (never contracted)
+template <bool RES>
+__device__ __forceinline__ float kept_sum(float x, float scale, float base) {
+  const float kept = __fmul_rn(x, scale);
+  return RES ? __fadd_rn(kept, base) : kept;
+}
+
 // Any addresses and strides.  One thread: the four elements of one counter block.
 template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs a) {
@@ -44,7 +54,7 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs a) {
       if (4 * b + e >= n) break;
       const float base = RES ? to_float<T>(res[row * a.residual_stride + col]) : 0.f;
       const float v = a.rate.none ? 0.f : to_float<T>(x[row * a.x_stride + col]);
-      y[4 * b + e] = T(a.rate.keep(w[e]) ? fmaf(v, a.rate.scale, base) : base);
+      y[4 * b + e] = T(a.rate.keep(w[e]) ? kept_sum<RES>(v, a.rate.scale, base) : base);
       if (++col == a.cols) { col = 0; ++row; }
     }
   }
@@ -96,7 +106,7 @@ struct DropTile {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float b = RES ? base[4 * q + e] : 0.f;
-        f[4 * q + e] = a.rate.keep(words[e]) ? fmaf(f[4 * q + e], a.rate.scale, b) : b;
+        f[4 * q + e] = a.rate.keep(words[e]) ? kept_sum<RES>(f[4 * q + e], a.rate.scale, b) : b;
       }
     }
     return floats_to_piece(f);
@@ -155,7 +165,7 @@ __global__ void __launch_bounds__(NT, 1) dropout_flat_kernel(const DropoutArgs a
     const float base = RES ? to_float<T>(static_cast<const T*>(a.residual)[e]) : 0.f;
     const bool keep = a.rate.keep(lane == 0 ? w.x : lane == 1 ? w.y : lane == 2 ? w.z : w.w);
     const float last = a.rate.none ? 0.f : to_float<T>(static_cast<const T*>(a.x)[e]);
-    static_cast<T*>(a.y)[e] = T(keep ? fmaf(last, a.rate.scale, base) : base);
+    static_cast<T*>(a.y)[e] = T(keep ? kept_sum<RES>(last, a.rate.scale, base) : base);
   }
 }
 

@@ -3,7 +3,8 @@
 //     with u = (z - mean) * rstd and g = dy * weight:
 //     dz = (g - mean(g) - u * mean(g * u)) * rstd [+ the gradient that reaches z from elsewhere]
 //     dx = keep ? dz / (1 - p) : 0, dresidual = dz, dweight = sum over rows of dy * u, dbias = sum over rows of dy
-// Statistics, sums and gradients are held in fp32; every output is rounded once.  The forward pass normalises the unrounded
+// Statistics, sums and gradients are held in fp32; every output is rounded once.  What the dropout keeps is rounded to fp32
+// before the residual is added, as in hyc_dropout.cu.  The forward pass normalises the unrounded
 // sum; the backward pass starts from z as it was stored.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -269,10 +270,10 @@ __device__ __forceinline__ void ln_drop(Philox& gen, const DropRate& rate, unsig
   const f32x2 scale = f2_both(rate.scale);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float lo, hi, b0 = 0.f, b1 = 0.f;
-    f2_split(BASE ? f2_fma(x[i], scale, base[i]) : f2_mul(x[i], scale), lo, hi);
-    if (BASE) f2_split(base[i], b0, b1);
-    x[i] = f2_make(keep[2 * i] ? lo : b0, keep[2 * i + 1] ? hi : b1);
+    float lo, hi;
+    f2_split(f2_mul(x[i], scale), lo, hi);
+    x[i] = f2_make(keep[2 * i] ? lo : 0.f, keep[2 * i + 1] ? hi : 0.f);
+    if (BASE) x[i] = f2_add(x[i], base[i]);            // behind the choice: next to each other the two packed ones become an FMA
   }
 }
 

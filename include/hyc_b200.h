@@ -317,9 +317,9 @@ int hyc_rope(void* q, void* k, const float* cos_sin, int64_t tokens, int32_t seq
  * Capturable: every replay of a recorded graph takes new numbers. */
 int hyc_rng_take(int64_t* state, int64_t* used, void* stream);
 
-/* y = residual + (kept ? x / (1 - p) : 0), in fp32, rounded once; residual may be NULL.  What is dropped is selected
- * away: infinities and NaN there do not reach y.  The backward pass is the same call on the gradient with residual =
- * NULL and the same rng. */
+/* y = residual + (kept ? x * (1 / (1 - p)) : 0): the factor, the product and the sum each rounded to fp32, the sum then
+ * once to dtype; residual may be NULL.  What is dropped is selected away: infinities and NaN there do not reach y.  The
+ * backward pass is the same call on the gradient with residual = NULL and the same rng. */
 typedef struct {
   int64_t rows, cols;
   int32_t dtype;           /* hyc_dtype of x, residual, y */

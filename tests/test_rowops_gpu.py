@@ -97,6 +97,26 @@ def test_dropout_of_unaligned_and_strided_tensors(ops, dtype, offsets):
     _near(ops.dropout(x[:1].cuda().expand(33, 40), 0.3, _rng().cuda()), *ro.dropout(one, 0.3, keep), "one row, seen 33 times")
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("p", [0.1, 0.05, 0.3])
+@pytest.mark.parametrize("rows,cols,offset", [(64, 768, 0), (3, 1001, 0), (64, 768, 1), (3000, 2048, 0)])
+def test_kept_values_are_rounded_before_the_residual_is_added(ops, dtype, p, rows, cols, offset):
+    """Each of product and sum is one IEEE operation, so the results are known to the bit.  Half of the residuals are what the
+    kept value is taken from (sums of exactly zero in fp32), and the inputs have few digits (sums on ties of bf16)."""
+    x = torch.randint(-255, 256, (rows, cols), generator=_gen(1)).float().mul_(9.0 / 64).to(dtype)
+    scale = torch.tensor(1.0 / (1.0 - p), dtype=F32)
+    away = torch.rand((rows, cols), generator=_gen(2)) < 0.5
+    res = torch.where(away, -(x.float() * scale), _randn((rows, cols), F32, 3, 8.0)).to(dtype)
+    keep = ro.keep_mask(11, 5, p, x.shape)
+    z = torch.where(keep, x.float() * scale, torch.zeros(())) + res.float()
+    if dtype == F32:
+        assert bool((z[away & keep] == 0).all())
+    got = ops.dropout(_offset(x, offset), p, _rng().cuda(), residual=_offset(res, offset))
+    assert torch.equal(got.cpu(), z.to(dtype))
+    out = ops.layer_norm(_offset(x, offset), None, None, residual=_offset(res, offset), p=p, rng=_rng().cuda())
+    assert torch.equal(out.z.cpu(), z.to(dtype))
+
+
 def test_dropout_of_nothing(ops):
     for shape in ((0,), (0, 8), (5, 0), (2, 0, 3)):
         x = torch.empty(shape, dtype=BF16, device="cuda")
