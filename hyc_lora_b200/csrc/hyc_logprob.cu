@@ -278,7 +278,7 @@ __device__ __forceinline__ float lp_lost(float m, float c, bool far) { return fa
 template <typename T>
 __device__ __noinline__ void lp_pick_slowly(const LpRow r, int vocab, int top, unsigned long long* best, unsigned long long* out) {
   constexpr int kPiece = 16 / sizeof(T);
-  unsigned long long before = ~0ull;
+  unsigned long long before = 0;            // the last turn's; the first has no upper bound (a NaN at index 0 has the largest key)
   for (int k = 0; k < top; ++k) {
     unsigned long long key = 0;
     for (int i = threadIdx.x; i < r.pieces; i += blockDim.x) {
@@ -290,7 +290,7 @@ __device__ __noinline__ void lp_pick_slowly(const LpRow r, int vocab, int top, u
       for (int e = 0; e < kPiece; ++e) {
         if (e0 + e < 0 || e0 + e >= vocab) continue;
         const unsigned long long q = lp_key(f[e], e0 + e);
-        if (q < before && q > key) key = q;
+        if ((k == 0 || q < before) && q > key) key = q;
       }
     }
 #pragma unroll

@@ -565,6 +565,33 @@ def test_logprobs_with_nan_and_infinity(ops, vocab):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [1, 4, 20, 32, 300, 3001, 40000, 100001])
+@pytest.mark.parametrize("where", ["first", "all", "ends", "both signs"])
+def test_logprobs_nan_is_an_alternative_wherever_it_stands(ops, dtype, vocab, where):
+    """A NaN stands above +inf, the lower index first among several; every index lies in the vocabulary, also where all of it
+    is asked for."""
+    x, t = _logit_inputs(4, vocab, dtype, 3)
+    if where == "first":
+        x[:, 0] = float("nan")
+    elif where == "all":
+        x[:] = float("nan")
+    elif where == "ends":
+        x[:, vocab - 1] = float("nan")
+        x[1, 0] = float("nan")
+        x[2, vocab // 2] = INF
+    else:
+        x[:, 0] = -torch.tensor(float("nan"))
+        x[:, vocab // 2] = float("nan")
+    x[3] = _randn((vocab,), dtype, 5)                         # a row without
+    rank = torch.where(x.isnan(), torch.full_like(x, INF, dtype=torch.float64), x.double().clamp_max(1e300))
+    order = torch.sort(rank, dim=1, descending=True, stable=True).indices
+    for top in sorted({1, min(5, vocab), min(32, vocab)}):
+        out = ops.token_logprobs(x.cuda(), t.cuda(), entropy=True, top=top)
+        assert torch.equal(out.top_index.cpu(), order[:, :top]), top
+        assert bool(out.top_logprob[:3].isnan().all()) and not bool(out.top_logprob[3].isnan().any())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("shift", [1000.0, -30000.0, 1.04e6, -1.2e6, 3e9, 1e20, -1e29, 1e31, -1e36])
 @pytest.mark.parametrize("rows,vocab", [(6, 1000), (6, 33000), (700, 2100)])
 def test_logprobs_of_logits_far_from_zero(ops, dtype, shift, rows, vocab):
