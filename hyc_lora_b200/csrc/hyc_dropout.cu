@@ -179,7 +179,8 @@ static void run_dropout_flat(const DropoutArgs& a, cudaStream_t stream) {
   auto kernel = dropout_flat_kernel<T, RES, U, NT>;
   const long long blocks = a.cols / (NT * U * (16 / sizeof(T))) + 1;
   static PerDevice resident;
-  const long long most = resident.get([&] { return resident_grid(kernel, NT, 0, 1 << 20); });
+  const int held = resident.get([&] { return held_at_once(kernel, NT, 0); });
+  const long long most = held ? held : sm_count();
   kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), NT, 0, stream>>>(a);
 }
 

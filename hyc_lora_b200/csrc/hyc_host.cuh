@@ -146,7 +146,8 @@ inline int resident_grid(K kernel, int threads, uint32_t smem_bytes, int grid) {
   return grid > cap ? static_cast<int>(cap) : grid;
 }
 
-// A positive number worked out once per device (what an occupancy query answers, an attribute that has been set).
+// A positive number worked out once per device.  What is kept may depend on the device and the kernel alone, not on the tuning
+// setting; a 0 (a query that failed) is not kept, the next call asks again.
 struct PerDevice {
   std::atomic<int> value[64];
   template <typename F>
@@ -161,6 +162,18 @@ struct PerDevice {
     return v;
   }
 };
+
+// CTAs of a kernel that the current device holds at once, whatever the tuning setting; 0 where the query fails.  A persistent
+// kernel launches this many, one per SM where it is not known.
+template <typename K>
+inline int held_at_once(K kernel, int threads, uint32_t smem_bytes) {
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem_bytes) != cudaSuccess || per_sm < 1) {
+    cudaGetLastError();
+    return 0;
+  }
+  return sm_count() * per_sm;
+}
 
 template <typename K>
 inline int set_smem(K kernel, uint32_t bytes) {

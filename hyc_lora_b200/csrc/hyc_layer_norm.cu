@@ -736,13 +736,15 @@ static bool misaligned(const void* p, uintptr_t bytes) { return reinterpret_cast
 static bool rows_aligned(const void* p, long long stride, uintptr_t es) { return !p || (aligned16(p) && stride * es % 16 == 0); }
 
 // CTAs of a kernel that the device holds at once, with the shared memory it asks for allowed first (without the attribute the
-// limit counts static shared memory too); 0: refused.  Worked out once per device and kernel.
+// limit counts static shared memory too); 0: that was refused.  Worked out once per device and kernel.
 template <typename K>
 static int ln_resident(PerDevice& cache, K kernel, int threads, uint32_t smem) {
-  return cache.get([&] {
-    if (smem > 32 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return 0;
-    return resident_grid(kernel, threads, smem, 1 << 20);
+  bool allowed = true;
+  const int held = cache.get([&] {
+    allowed = smem <= 32 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess;
+    return allowed ? held_at_once(kernel, threads, smem) : 0;
   });
+  return held || !allowed ? held : sm_count();
 }
 
 // Rows ahead by what shared memory holds beside `table` bytes: two CTAs of 256 threads an SM, or one of 512.  Fewer than

@@ -943,10 +943,10 @@ static int check_logprob(int64_t rows, int32_t vocab, int32_t dtype, int64_t seq
   return HYC_OK;
 }
 
-// clusters of `ranks` CTAs that the device holds at once
+// clusters of `ranks` CTAs that the device holds at once; 0 where the query fails
 template <typename K>
 static int resident_clusters(K kernel, int threads, int ranks) {
-  if (ranks == 1) return resident_grid(kernel, threads, 0, 1 << 20);
+  if (ranks == 1) return held_at_once(kernel, threads, 0);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -955,7 +955,7 @@ static int resident_clusters(K kernel, int threads, int ranks) {
   int n = 0;
   if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
     cudaGetLastError();
-    return sm_count() / ranks;
+    return 0;
   }
   return n;
 }
@@ -964,7 +964,8 @@ template <typename T, int THREADS, bool ENT, bool TOP, bool CLUSTER>
 static int run_logprob(const LogprobArgs& a, int ranks, cudaStream_t stream) {
   auto kernel = logprob_kernel<T, THREADS, ENT, TOP, CLUSTER>;
   static PerDevice resident[4];            // by cluster size
-  const long long most = resident[ranks == 8 ? 3 : ranks >> 1].get([&] { return resident_clusters(kernel, THREADS, ranks); });
+  const int held = resident[ranks == 8 ? 3 : ranks >> 1].get([&] { return resident_clusters(kernel, THREADS, ranks); });
+  const long long most = held ? held : sm_count() / ranks;
   const long long clusters = a.rows < most ? a.rows : most;
   cudaError_t e;
   if (CLUSTER) {

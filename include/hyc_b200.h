@@ -124,7 +124,9 @@ uint64_t hyc_launch_count(void);
 /* Optional launch tuning for experiments (0 = library default): threads per row-CTA, staging
  * depth, resident CTAs per SM.  The setting is PROCESS-GLOBAL and unsynchronised: it changes the
  * launches of every thread and stream from then on, so set it before the threads that launch are
- * started (or not at all); every other entry point keeps no mutable state. */
+ * started (or not at all).  The row operators (hyc_dropout, hyc_layer_norm*, hyc_token_logprobs*) do
+ * not take it; what they keep between calls is how many CTAs of each kernel a device holds.  Beside
+ * hyc_debug_wait and hyc_select_channels_noalloc (below) no other entry point keeps mutable state. */
 int hyc_set_tuning(int threads, int stages, int ctas_per_sm);
 
 /* Test hook for the give-up path of the bounded waits, PROCESS-GLOBAL like hyc_set_tuning and 0/0 in

@@ -964,3 +964,32 @@ def test_tensors_of_two_devices_are_refused(ops):
         ops.dropout(x, 0.1, _rng())
     with pytest.raises(RuntimeError, match="no CPU path"):
         ops.layer_norm(x, None, None, p=0.1, rng=_rng())
+
+
+def test_the_tuning_setting_leaves_the_row_operators_alone(ops):
+    """A process that tunes the compression kernels before its first call of a row operator, and one that does not: the sums of
+    the parameter gradients are taken in the same order, which is that of the CTAs that the device holds."""
+    import subprocess
+    import sys
+    code = """
+import sys
+import torch
+from hyc_lora_b200 import _lib, rowops as o
+tuned = sys.argv[1] == 'tuned'
+digests = []
+for dtype, cols in ((torch.bfloat16, 768), (torch.float32, 1024), (torch.bfloat16, 4096)):
+    g = torch.Generator().manual_seed(cols)
+    dy, z = (torch.randn(5000, cols, generator=g).to(dtype).cuda() for _ in range(2))
+    mean, rstd = torch.zeros(5000, device='cuda'), torch.ones(5000, device='cuda')
+    for ctas in ((2, 0) if tuned else (0, 0)):
+        assert _lib.lib.hyc_set_tuning(0, 0, ctas) == 0
+        for t in o.layer_norm_bwd(dy, z, None, mean, rstd, param_dtype=torch.float32)[2:]:
+            digests.append(t.view(torch.int32).long().mul(torch.arange(1, cols + 1, device='cuda')).sum().item())
+print(digests)
+"""
+    def digests(how):
+        done = subprocess.run([sys.executable, "-c", code, how], capture_output=True, text=True, timeout=300, cwd=ROOT)
+        assert done.returncode == 0, done.stderr[-2000:]
+        return done.stdout
+
+    assert digests("tuned") == digests("plain")
