@@ -221,9 +221,13 @@ class DecoderLM(nn.Module):
     def score(self, ids, entropy: bool = False, top: int = 0):
         """Log probability of every token after the first (``logprob[:, t]`` is that of ``ids[:, t + 1]``, 0 at the end), with
         the entropy of the model's distribution and its ``top`` alternatives at every position: a
-        :class:`~hyc_lora_b200.rowops.TokenLogprobs`."""
+        :class:`~hyc_lora_b200.rowops.TokenLogprobs`.  Where compression operators are installed their calibration stays what
+        it was, so scoring before or between training steps does not change them."""
+        from ..operators._common import calibration_kept
         from ..rowops import token_logprobs
-        return token_logprobs(self.logits(ids), self._next(ids), entropy=entropy, top=top)
+        with calibration_kept(self):
+            logits = self.logits(ids)
+        return token_logprobs(logits, self._next(ids), entropy=entropy, top=top)
 
     def forward(self, ids):
         logits = self.logits(ids)

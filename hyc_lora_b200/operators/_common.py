@@ -3,6 +3,7 @@ mean of the reference, the options of the channel mode and the one helper that
 compresses an activation for backward in either mode."""
 from __future__ import annotations
 
+import contextlib
 import weakref
 from typing import Optional
 
@@ -270,3 +271,42 @@ def load_calibration_state_dict(module, state: dict) -> None:
         if name in state and hasattr(module, name):
             c = getattr(module, name).calib
             c.score, c.channels = state[name]["score"], state[name]["channels"]
+
+
+@contextlib.contextmanager
+def calibration_kept(model):
+    """Forward passes inside leave the calibration of ``model``'s sites as they found it: statistics, channel choices, pool
+    densities, learnt readers of norm outputs and the call counts that say when calibration ends.  For passes over other data
+    than what is trained on (scoring), whose activations are not saved for any backward pass."""
+    global _last_norm_output
+    lists, attributes = [], []
+    for module in model.modules():
+        if not hasattr(module, "iteration"):
+            continue
+        kept = {"iteration": module.iteration}
+        for name in ("static_value", "static_value_1", "static_value_2"):
+            if hasattr(module, name):
+                value = kept[name] = getattr(module, name)
+                if isinstance(value, list):
+                    lists.append((value, list(value), dict(getattr(value, "cache", ()))))
+        attributes.append((module, kept, False))
+        for name in ("site", "site_1", "site_2"):
+            if hasattr(module, name):
+                options = getattr(module, name)
+                attributes.append((options, dict(vars(options)), True))
+                attributes.append((options.calib, dict(vars(options.calib)), True))
+    shared, last_norm_output = list(_shared), _last_norm_output
+    try:
+        yield
+    finally:
+        for owner, kept, whole in attributes:
+            if whole:
+                vars(owner).clear()
+            vars(owner).update(kept)
+        for value, items, cache in lists:
+            value[:] = items
+            if isinstance(value, StaticList):
+                value.cache.clear()
+                value.cache.update(cache)
+        _shared[:] = shared
+        _last_norm_output = last_norm_output

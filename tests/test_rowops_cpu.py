@@ -240,6 +240,50 @@ def test_hosts_build_with_and_without_the_row_operators(lib):
     assert torch.isfinite(plain(ids, labels))
 
 
+def test_calibration_kept_puts_every_site_back(lib):
+    from hyc_lora_b200.operators import _common as co
+    from hyc_lora_b200.operators.efficient_gemm import EfficientMemoryGEMM
+    from hyc_lora_b200.operators.efficient_linear import EfficientMemoryLinear
+    from hyc_lora_b200.operators.efficient_softmax import EfficientMemorySoftmax
+    model = torch.nn.ModuleList([EfficientMemoryLinear(128, 8, rank=0, outlier_mode="channel"), EfficientMemoryGEMM(), EfficientMemorySoftmax(0.05)])
+    linear, gemm, softmax = model
+    one = [torch.ones(2, 2) for _ in range(4)]
+    co.update_static(gemm.static_value_1, 0, *one)
+    gemm.static_value_1.cache["pool_density"] = 0.25
+    gemm.iteration = 1
+    linear.site.calib.score = torch.arange(4.0)
+    before = [co.calibration_state_dict(m) for m in model]
+
+    def pass_over_other_data():
+        for m in model:
+            m.iteration += 2
+        for static in (linear.static_value, gemm.static_value_1, gemm.static_value_2):
+            co.update_static(static, 0, *(2 * t for t in one))
+            static.cache["pool_density"] = 0.5
+        softmax.static_value = torch.ones(())
+        linear.site.calib.score, linear.site.calib.channels = torch.zeros(4), torch.zeros(1, dtype=torch.int32)
+        linear.site.calib._compared = linear.site.calib.channels
+        linear.site.output_format, linear.site.pending_output = (4, 0, 0, linear.site.calib), object()
+        co._shared.insert(0, "a record")
+        co._last_norm_output = "an output"
+
+    shared, last, static = list(co._shared), co._last_norm_output, gemm.static_value_1
+    for fails in (False, True):
+        try:
+            with co.calibration_kept(model):
+                pass_over_other_data()
+                assert linear.iteration == 2
+                if fails:
+                    raise KeyError
+        except KeyError:
+            pass
+        after = [co.calibration_state_dict(m) for m in model]
+        assert str(before) == str(after)
+        assert gemm.static_value_1 is static and static.cache == {"pool_density": 0.25} and linear.static_value.cache == {}
+        assert linear.site.output_format is None and linear.site.pending_output is None and not hasattr(linear.site.calib, "_compared")
+        assert co._shared == shared and co._last_norm_output is last
+
+
 # ------------------------------------------------------------------------------------------------ orderings, read from the source
 
 def _kernel_bodies(text):

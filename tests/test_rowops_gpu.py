@@ -862,6 +862,54 @@ def test_decoder_host_with_the_fused_loss(ops):
     assert torch.equal(got.top_index.reshape(-1, 3).cpu(), ref["top_index"])
 
 
+@pytest.mark.parametrize("mode", ["element", "channel"])
+@pytest.mark.parametrize("scored_before", [0, 1, 2, 3])
+def test_scoring_leaves_the_calibration_alone(ops, mode, scored_before):
+    """A model with compression operators that is scored on other text before its training step ``scored_before``, and a copy that
+    is not: the same calibration and, to the bit, the same losses and gradients."""
+    from hyc_lora_b200 import synthetic
+    from hyc_lora_b200.hosts.llama import DecoderConfig, DecoderLM
+    from hyc_lora_b200.hosts.replace import replace_module, uniform_config
+    from hyc_lora_b200.operators._common import calibration_state_dict
+    cfg = DecoderConfig(hidden=512, layers=2, heads=4, kv_heads=2, ffn=1408, vocab=1001, lora_r=16, base_quant="nf4", fused_loss=True)
+    model = DecoderLM(cfg, seed=1)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for n, q in model.named_parameters():
+        if "lora_B" in n:
+            q.data.normal_(0, 0.05, generator=gen)
+    extra = dict(outlier_mode="channel", rotate=64) if mode == "channel" else {}
+    assert replace_module(model, uniform_config(outlier_ratio=0.02), extra) > 0
+    other = copy.deepcopy(model)
+    for step in range(5):
+        ids = synthetic.token_ids(10 + step, 2, 64, cfg.vocab).cuda()
+        results = []
+        for m in (model, other):
+            if m is model and step >= scored_before:
+                text = synthetic.token_ids(90 + step, 3, 40, cfg.vocab).cuda()
+                got = m.score(text, entropy=True, top=2)
+                assert torch.equal(got.logprob, m.score(text).logprob)
+            m.zero_grad(set_to_none=True)
+            loss = m(ids)
+            loss.backward()
+            results.append((loss.item(), {n: q.grad for n, q in m.named_parameters() if q.grad is not None}))
+        (a, ga), (b, gb) = results
+        assert a == b and ga.keys() == gb.keys() and len(ga) > 0
+        assert all(torch.equal(ga[n], gb[n]) for n in ga), step
+    for (n, p), (_, q) in zip(model.named_modules(), other.named_modules()):
+        if hasattr(p, "iteration"):
+            assert p.iteration == 5 and _same(calibration_state_dict(p), calibration_state_dict(q)), n
+
+
+def _same(a, b):
+    if torch.is_tensor(a):
+        return torch.is_tensor(b) and torch.equal(a, b)
+    if isinstance(a, dict):
+        return a.keys() == b.keys() and all(_same(a[k], b[k]) for k in a)
+    if isinstance(a, (list, tuple)):
+        return len(a) == len(b) and all(_same(p, q) for p, q in zip(a, b))
+    return a == b
+
+
 def test_encoder_host_with_hidden_dropout(ops):
     """The whole host with its dropouts against the same host with the masks applied by tensor ops, and a recorded step."""
     from hyc_lora_b200.hosts.roberta import EncoderClassifier, EncoderConfig
