@@ -74,7 +74,7 @@ class CounterDropoutFunc(torch.autograd.Function):
 class EfficientMemoryCounterDropout(torch.nn.Module):
     """Dropout from a counter-based generator, with an optional residual added in the same kernel.
 
-    ``forward(x, residual=None, rng=None)``.  The state (seed and call number) is a buffer on the device: it moves with the
+    ``forward(x, residual=None, rng=None)``; the residual has x's shape and dtype, in training and in evaluation.  The state (seed and call number) is a buffer on the device: it moves with the
     module, is saved with it, and a step recorded into a CUDA graph draws a new mask at every replay.  Copies of a module
     draw the same masks as the original; give ranks that should differ seeds of their own.  A forward pass that is run again
     by activation checkpointing has to see its first mask: take ``rng = module.take()`` outside the checkpointed function
@@ -92,7 +92,10 @@ class EfficientMemoryCounterDropout(torch.nn.Module):
 
     def forward(self, x, residual=None, rng=None):
         if not self.training or self.p == 0.0:
-            return x if residual is None else residual + x
+            if residual is None:
+                return x
+            rowops.check_like("residual", residual, x)         # the same calls as with dropout
+            return residual + x
         return CounterDropoutFunc.apply(x, residual, self.p, self.take() if rng is None else rng)
 
     def extra_repr(self):

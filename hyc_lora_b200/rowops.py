@@ -101,7 +101,7 @@ def _check_rng(rng: Optional[torch.Tensor]):
         raise ValueError("rng must be a contiguous int64 tensor of two values: seed and call number")
 
 
-def _like(name: str, t: torch.Tensor, x: torch.Tensor):
+def check_like(name: str, t: torch.Tensor, x: torch.Tensor):
     if t.shape != x.shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(x.shape)}")
     if t.dtype != x.dtype:
@@ -150,7 +150,7 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: Optional[tor
         code = _dtype_code(x)
     x_stride = residual_stride = at_residual = 0
     if residual is not None:
-        _like("residual", residual, x)
+        check_like("residual", residual, x)
     if x.is_contiguous() and (residual is None or residual.is_contiguous()):
         rows, cols = 1, x.numel()
     else:
@@ -187,7 +187,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
         _check_rng(rng)
         at_rng = rng.data_ptr()
     if residual is not None:
-        _like("residual", residual, x)
+        check_like("residual", residual, x)
         residual, residual_stride = _rows(residual)
         at_residual = residual.data_ptr()
     x, x_stride = _rows(x)
@@ -214,7 +214,7 @@ def layer_norm_bwd(dy: torch.Tensor, z: torch.Tensor, weight: Optional[torch.Ten
         raise ValueError("layer_norm_bwd takes tensors of at least one dimension")
     cols = dy.shape[-1]
     _check_params(weight, None, cols)
-    _like("z", z, dy)
+    check_like("z", z, dy)
     code = _CODES.get(dy.dtype)
     if code is None:
         code = _dtype_code(dy)
@@ -227,7 +227,7 @@ def layer_norm_bwd(dy: torch.Tensor, z: torch.Tensor, weight: Optional[torch.Ten
         _check_rng(rng)
         at_rng = rng.data_ptr()
     if dz is not None:
-        _like("dz", dz, dy)
+        check_like("dz", dz, dy)
         dz, dz_stride = _rows(dz)
         at_dz = dz.data_ptr()
     dy, dy_stride = _rows(dy)

@@ -217,6 +217,21 @@ def test_modules_validate_and_keep_their_state(lib):
         n(torch.zeros(2, 9))
 
 
+@pytest.mark.parametrize("p,training", [(0.1, False), (0.0, True), (0.0, False)])
+def test_counter_dropout_takes_the_same_residuals_without_dropping(lib, p, training):
+    """With dropout the kernel refuses a residual of another shape or dtype; so does the sum that takes its place."""
+    from hyc_lora_b200.operators.efficient_dropout import EfficientMemoryCounterDropout
+    m = EfficientMemoryCounterDropout(p).train(training)
+    x = torch.ones(3, 4)
+    for bad in (torch.ones(1, 4), torch.ones(4), torch.ones(3, 1), torch.ones(2, 3, 4)):
+        with pytest.raises(ValueError, match="residual has shape"):
+            m(x, bad)
+    for bad in (torch.ones(3, 4, dtype=torch.bfloat16), torch.ones(3, 4, dtype=torch.float64)):
+        with pytest.raises(TypeError, match="residual is"):
+            m(x, bad)
+    assert torch.equal(m(x, 2 * x), 3 * x) and m(x) is x
+
+
 def test_replacement_leaves_the_row_operators_alone(lib):
     from hyc_lora_b200.hosts.replace import replace_module, uniform_config
     from hyc_lora_b200.operators.efficient_dropout import EfficientMemoryCounterDropout
