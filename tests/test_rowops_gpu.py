@@ -254,6 +254,38 @@ def test_layer_norm_matches_the_plain_form(ops, cols, dtype, params, p, with_res
     assert got[2].dtype == params and got[3].dtype == params
 
 
+# Rows enough for every group of threads to take several: the forward pass with rows ahead in shared memory (from 4 rows per group
+# and SM on: 4736, 1184 and 592 rows by the width), the sums of the parameter gradients over a group's rows, over groups and CTAs.
+# Widths that fill their slots exactly (bounds are left out), that do not, and that are no multiple of eight.
+MANY_ROWS = [(4740, 256), (4800, 248), (5000, 768), (5000, 760), (4800, 767), (5000, 1024), (4900, 1000), (1300, 2048), (1300, 1800),
+             (1250, 2041), (1300, 4096), (1300, 4000), (700, 4095), (700, 6144), (700, 6000), (700, 8192), (700, 8184), (620, 8191),
+             (700, 11008), (600, 12288), (600, 12287), (600, 16384), (600, 16000)]
+
+
+@pytest.mark.parametrize("rows,cols", MANY_ROWS)
+@pytest.mark.parametrize("dtype,params", [(BF16, F32), (F32, BF16)])
+def test_layer_norm_of_many_rows(ops, rows, cols, dtype, params):
+    x, w, b = _norm_inputs(rows, cols, dtype, params, cols)
+    res, dy, dz = (_randn((rows, cols), dtype, s) for s in (9, 7, 8))
+    keep = ro.keep_mask(11, 5, 0.2, x.shape)
+    rng = _rng().cuda()
+    out = ops.layer_norm(x.cuda(), w.cuda(), b.cuda(), 1e-5, residual=res.cuda(), p=0.2, rng=rng)
+    for name, got, a, bound in zip(out._fields, out, *ro.layer_norm(x, w, b, 1e-5, res, 0.2, keep)):
+        _near(got, a, bound, name)
+    mean, rstd = out.mean.cpu(), out.rstd.cpu()
+    got = ops.layer_norm_bwd(dy.cuda(), out.z, w.cuda(), out.mean, out.rstd, p=0.2, rng=rng, dz=dz.cuda())
+    for name, a, v, bound in zip(("dx", "dresidual", "dweight", "dbias"), got, *ro.layer_norm_bwd(dy, out.z.cpu(), w, mean, rstd, 0.2, keep, dz, params)):
+        _near(a, v, bound, name)
+    # neither dropout nor a second gradient of the sum, no parameters
+    out = ops.layer_norm(x.cuda(), None, None, 1e-5)
+    for name, got, a, bound in zip(out._fields, out, *ro.layer_norm(x, None, None, 1e-5)):
+        _near(got, a, bound, name)
+    got = ops.layer_norm_bwd(dy.cuda(), out.z, None, out.mean, out.rstd, param_dtype=F32)
+    for name, a, v, bound in zip(("dx", "dresidual", "dweight", "dbias"), got,
+                                 *ro.layer_norm_bwd(dy, x, None, out.mean.cpu(), out.rstd.cpu(), param_dtype=F32)):
+        _near(a, v, bound, name)
+
+
 @pytest.mark.parametrize("rows", [0, 1, 2, 3, 31, 149, 1000, 5000])
 @pytest.mark.parametrize("cols", [96, 99, 2056])
 def test_layer_norm_row_counts(ops, rows, cols):
