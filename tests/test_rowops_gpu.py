@@ -894,6 +894,32 @@ def test_decoder_host_with_the_fused_loss(ops):
     assert torch.equal(got.top_index.reshape(-1, 3).cpu(), ref["top_index"])
 
 
+def test_fused_loss_hands_the_same_gradient_to_the_logits(ops):
+    """Both losses give the logits' gradient in bf16, rounded once from fp32: two values that are each within half a step of the
+    formula's are at most one step (2^-7 of the value) apart; 2^-20 of it is for the fp32 arithmetic, softmax and quotient."""
+    from hyc_lora_b200 import synthetic
+    from hyc_lora_b200.hosts.llama import DecoderConfig, DecoderLM
+    cfg = DecoderConfig(hidden=512, layers=1, heads=4, kv_heads=2, ffn=1408, vocab=1001, lora_r=16, base_quant="nf4")
+    model = DecoderLM(cfg, seed=1)
+    ids = synthetic.token_ids(3, 3, 33, cfg.vocab).cuda()
+    kept = []
+    model.lm_head.register_forward_hook(lambda module, args, out: (out.retain_grad(), kept.append(out))[0])
+    grads = []
+    for fused in (False, True):
+        model.zero_grad(set_to_none=True)
+        model.config.fused_loss = fused
+        model(ids).backward()
+        grads.append({n for n, q in model.named_parameters() if q.grad is not None})
+    assert grads[0] == grads[1] and len(grads[0]) > 0
+    plain, fused = kept
+    assert torch.equal(plain, fused) and plain.grad.dtype == fused.grad.dtype == BF16
+    a, b = plain.grad.double(), fused.grad.double()
+    assert bool((b[:, -1] == 0).all()) and bool(((a - b).abs() <= (2.0 ** -7 + 2.0 ** -20) * torch.minimum(a.abs(), b.abs())).all())
+    x, t = plain.detach().double()[:, :-1], ids[:, 1:]
+    want = (torch.softmax(x, -1) - torch.nn.functional.one_hot(t, cfg.vocab)) / t.numel()
+    assert bool(((b[:, :-1] - want).abs() <= (2.0 ** -8 + 2.0 ** -18) * want.abs()).all())
+
+
 @pytest.mark.parametrize("mode", ["element", "channel"])
 @pytest.mark.parametrize("scored_before", [0, 1, 2, 3])
 def test_scoring_leaves_the_calibration_alone(ops, mode, scored_before):
