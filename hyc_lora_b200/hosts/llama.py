@@ -225,7 +225,8 @@ class DecoderLM(nn.Module):
         it was, so scoring before or between training steps does not change them."""
         from ..operators._common import calibration_kept
         from ..rowops import token_logprobs
-        with calibration_kept(self):
+        # the sites tell tensors apart by their version counters, which tensors of an inference mode do not have
+        with torch.inference_mode(False), torch.no_grad(), calibration_kept(self):
             logits = self.logits(ids)
         return token_logprobs(logits, self._next(ids), entropy=entropy, top=top)
 

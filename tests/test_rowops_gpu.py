@@ -958,6 +958,28 @@ def test_scoring_leaves_the_calibration_alone(ops, mode, scored_before):
             assert p.iteration == 5 and _same(calibration_state_dict(p), calibration_state_dict(q)), n
 
 
+@pytest.mark.parametrize("mode", ["none", "element", "channel"])
+def test_scoring_in_inference_mode(ops, mode):
+    """The very first call of a model in inference mode, then outside, then a training step: nothing made in the one is kept for
+    the others."""
+    from hyc_lora_b200 import synthetic
+    from hyc_lora_b200.hosts.llama import DecoderConfig, DecoderLM
+    from hyc_lora_b200.hosts.replace import replace_module, uniform_config
+    cfg = DecoderConfig(hidden=256, layers=2, heads=4, kv_heads=2, ffn=512, vocab=301, lora_r=16, rope_theta=9000.0, fused_loss=True)
+    model = DecoderLM(cfg, seed=1)
+    if mode != "none":
+        replace_module(model, uniform_config(outlier_ratio=0.02), dict(outlier_mode="channel", rotate=64) if mode == "channel" else {})
+    ids = synthetic.token_ids(3, 2, 48, cfg.vocab).cuda()
+    with torch.inference_mode():
+        got = model.score(ids.clone(), entropy=True, top=3)
+    want = model.score(ids, entropy=True, top=3)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    for _ in range(3):
+        model(ids).backward()
+    assert all(bool(q.grad.isfinite().all()) for q in model.parameters() if q.requires_grad)
+
+
 def _same(a, b):
     if torch.is_tensor(a):
         return torch.is_tensor(b) and torch.equal(a, b)
