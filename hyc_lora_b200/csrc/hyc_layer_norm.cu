@@ -835,7 +835,10 @@ static int run_ln_bwd(LnBwdArgs a, cudaStream_t stream) {
     cfg.gridDim = dim3((2 * a.cols + 31) / 32); cfg.blockDim = dim3(1024); cfg.stream = stream; cfg.attrs = &attr; cfg.numAttrs = 1;
     const cudaError_t f = cudaLaunchKernelEx(&cfg, ln_finish_kernel, a);
     HYC_LAUNCHED();
-    if (f != cudaSuccess) return cuda_fail(f, "ln_finish_kernel");
+    if (f != cudaSuccess) {
+      cudaGetLastError();                  // a refused launch is this call's error, not also the next one's
+      return cuda_fail(f, "ln_finish_kernel");
+    }
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? HYC_OK : cuda_fail(e, "ln_bwd_kernel");

@@ -1121,3 +1121,58 @@ print(digests)
         return done.stdout
 
     assert digests("tuned") == digests("plain")
+
+
+@pytest.mark.parametrize("which", ["clusters", "norm backward"])
+def test_a_refused_launch_is_reported_once(which):
+    """Launches into a stream whose capture has been invalidated (on the host, by a synchronisation inside it) are refused by the
+    runtime.  That call says so; the next one, on a stream in order, is not blamed for it.  In a process of its own: torch's
+    generator does not come out of an invalidated capture."""
+    import subprocess
+    import sys
+    code = """
+import ctypes as C
+import sys
+import torch
+from hyc_lora_b200 import _lib
+logits, stats = torch.ones(2, 40000, device='cuda'), torch.empty(2, 2, device='cuda')
+x, y, one, sums = (torch.ones(n, device='cuda') for n in (384, 384, 64, 768))
+rng = torch.tensor([1, 2], device='cuda')
+
+def dropout(stream):
+    a = _lib.HycDropoutArgs(rows=1, cols=384, dtype=_lib.HYC_F32, x=x.data_ptr(), y=y.data_ptr(), rng=rng.data_ptr(), p=0.5)
+    return _lib.lib.hyc_dropout(C.byref(a), stream)
+
+def norm_backward(stream):
+    a = _lib.HycLayerNormBwdArgs(rows=6, cols=64, dtype=_lib.HYC_F32, param_dtype=_lib.HYC_F32, dy=x.data_ptr(), dy_stride=64,
+                                 z=x.data_ptr(), z_stride=64, mean=one.data_ptr(), rstd=one.data_ptr(), dresidual=y.data_ptr(),
+                                 dbias=one.data_ptr(), partials=sums.data_ptr())
+    return _lib.lib.hyc_layer_norm_bwd(C.byref(a), stream)
+
+def clusters(stream):
+    a = _lib.HycLogprobArgs(logits=logits.data_ptr(), rows=2, row_stride=40000, seq=2, vocab=40000, dtype=_lib.HYC_F32, stats=stats.data_ptr())
+    return _lib.lib.hyc_token_logprobs(C.byref(a), stream)
+
+first = clusters if sys.argv[1] == 'clusters' else norm_backward
+good, broken, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+codes = [first(good.cuda_stream), dropout(good.cuda_stream)]
+good.synchronize()
+with torch.cuda.stream(broken):
+    graph.capture_begin(capture_error_mode='thread_local')
+    try:
+        broken.synchronize()
+        raise SystemExit('a capture outlived a synchronisation')
+    except RuntimeError:
+        pass
+    codes.append(first(broken.cuda_stream))
+    try:
+        graph.capture_end()
+    except RuntimeError:
+        pass
+codes += [dropout(good.cuda_stream), first(good.cuda_stream)]
+good.synchronize()
+print(codes)
+"""
+    done = subprocess.run([sys.executable, "-c", code, which], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert done.returncode == 0 and done.stdout.split("\n")[0] == "[0, 0, -8, 0, 0]", (done.stdout, done.stderr[-2000:])
