@@ -61,9 +61,10 @@ __global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs a) {
 }
 
 // One flat run of elements at 16-byte aligned addresses.  Persistent: a CTA takes tiles of U * NT pieces of 16 bytes and has the
-// next tile's loads in flight while it draws this tile's words.  Without a residual and in bf16 the generator's products (see
-// hyc_philox.cuh) bound it, else DRAM.  Many words per thread keep the multiplier fed: 16384 x 11008 bf16 takes 141 us (DRAM
-// alone: 112; the products alone: 97) with U = 8 and 256 threads, 143 with 384, 160 with 512; at 8192 x 11008 U = 8 takes 74 us,
+// next tile's loads in flight while it draws this tile's words.  Without a residual and in bf16 it stands between two
+// bounds that overlap in part, DRAM and the generator's products (see hyc_philox.cuh; their pipe is busy for 67 % of the time),
+// else at DRAM's.  Many words per thread keep the multiplier fed: 16384 x 11008 bf16 takes 141 us (DRAM alone: 112; the
+// products alone: 97) with U = 8 and 256 threads, 143 with 384, 160 with 512; at 8192 x 11008 U = 8 takes 74 us,
 // U = 4 80, U = 2 83.  With a residual 384 threads of U = 4 take 69 us at 16384 x 4096 (DRAM: 62), 256 threads 75.
 
 // eight bf16 values as fp32; both halves by byte permutes and masks, which leave the multiplier's pipe to the generator

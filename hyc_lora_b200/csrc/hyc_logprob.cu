@@ -1002,10 +1002,14 @@ static double lp_cost(long long rows, long long places, int extra) {
 // Threads per row.  A row's end (joining the sums, finding the alternatives) is a chain of latencies that only other CTAs of
 // the SM fill, so small CTAs -- more of them, each with more of a row per thread -- do better; large ones do where there are too
 // few rows for all places, or where they leave a fuller last round.  Measured, us, with 256 / 128 / 64 threads (bf16, 32000
-// tokens): with five alternatives and entropy 8192 rows 146 / 128 / 130, 4096 rows 76 / 66 / 74, 1000 rows 25 / 21 / 23, 300
-// rows 10 / 12 / 16; log probabilities only 8192 rows 105 / 96 / 91, 4096 rows 56 / 50 / 52, 300 rows 9 / 10 / 12; fp32, 1024
-// rows of 50265 with entropy 41 / 44 / 39.  The percentages below are these, less the rounds.  Rows of fewer than two chunks
-// take fewer threads in any case.
+// tokens): with five alternatives and entropy 8192 rows 146 / 126 / 126, 4096 rows 76 / 65 / 71, 1000 rows 24 / 24 / 23, 300
+// rows 10 / 12 / 16; log probabilities only 8192 rows 106 / 96 / 91, 4096 rows 55 / 50 / 50, 300 rows 9 / 10 / 12; fp32, 1024
+// rows of 50265 with entropy 41 / 44 / 39.  The percentages below are these, less the rounds: shares of the bytes of such rows,
+// by which the choice is within 2 % of the best of the three there.  A row's end does not grow with the vocabulary, so
+// elsewhere it is further off.  With alternatives: 8200 tokens, 4096 rows 53 / 36 / 28 (128 are taken; 35 % off at worst);
+// 131072 tokens, 1000 rows 61 / 78 / 90 (128, 27 %), 4096 rows 214 / 233 / 285 (128, 9 %); fp32, 32000 tokens, 1000 rows 33 /
+// 41 / 45 (128, 23 %).  Log probabilities only: 8200 tokens, 4096 rows 33 / 24 / 19 (128, 25 %), 131072 tokens, 1000 rows 50 /
+// 58 / 52 (64, 5 %).  Rows of fewer than two chunks take fewer threads in any case.
 template <typename T>
 static int lp_threads(const LogprobArgs& a, long long pieces) {
   if (pieces <= 2 * 32 * kLpChunk) return 32;
@@ -1021,7 +1025,8 @@ static int lp_threads(const LogprobArgs& a, long long pieces) {
   return best;
 }
 
-// Few long rows are spread over clusters, as far as a slice keeps two chunks and the SMs' places for CTAs go.
+// Few long rows are spread over clusters, as far as a slice keeps 512 pieces (two per thread, half a chunk: all of them are then
+// fetched under bounds) and four CTAs per SM go.
 template <typename T>
 static int launch_logprob(const LogprobArgs& a, cudaStream_t stream) {
   const long long pieces = (static_cast<long long>(a.vocab) * sizeof(T) + 15) / 16 + 1;
