@@ -74,12 +74,13 @@ class CounterDropoutFunc(torch.autograd.Function):
 class EfficientMemoryCounterDropout(torch.nn.Module):
     """Dropout from a counter-based generator, with an optional residual added in the same kernel.
 
-    ``forward(x, residual=None, rng=None)``; the residual has x's shape and dtype, in training and in evaluation.  The state (seed and call number) is a buffer on the device: it moves with the
-    module, is saved with it, and a step recorded into a CUDA graph draws a new mask at every replay.  Copies of a module
-    draw the same masks as the original; give ranks that should differ seeds of their own.  (Under torch's
-    DistributedDataParallel that takes ``broadcast_buffers=False``: by default it copies rank 0's buffers, this state among them,
-    to all ranks in front of every forward pass.  ``hyc_lora_b200.ddp`` exchanges gradients only.)  A forward pass that is run again
-    by activation checkpointing has to see its first mask: take ``rng = module.take()`` outside the checkpointed function
+    ``forward(x, residual=None, rng=None)``; the residual has x's shape and dtype, in training and in evaluation.  The state
+    (seed and call number) is a buffer on the device: it moves with the module, is saved with it, and a step recorded into a
+    CUDA graph draws a new mask at every replay.  Copies of a module draw the same masks as the original; give ranks that
+    should differ seeds of their own.  (Under torch's DistributedDataParallel that takes ``broadcast_buffers=False``: by
+    default it copies rank 0's buffers, this state among them, to all ranks in front of every forward pass.
+    ``hyc_lora_b200.ddp`` exchanges gradients only.)  A forward pass that is run again by activation checkpointing has to see
+    its first mask: take ``rng = module.take()`` outside the checkpointed function
     and hand it to ``forward``."""
 
     def __init__(self, p: float = 0.5, seed=None, device=None):
