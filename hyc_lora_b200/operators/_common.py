@@ -281,18 +281,19 @@ def calibration_kept(model):
     global _last_norm_output
     lists, attributes = [], []
     for module in model.modules():
-        if not hasattr(module, "iteration"):
+        own = vars(module)
+        if "iteration" not in own:
             continue
-        kept = {"iteration": module.iteration}
+        kept = {"iteration": own["iteration"]}
         for name in ("static_value", "static_value_1", "static_value_2"):
-            if hasattr(module, name):
-                value = kept[name] = getattr(module, name)
+            if name in own:
+                value = kept[name] = own[name]
                 if isinstance(value, list):
                     lists.append((value, list(value), dict(getattr(value, "cache", ()))))
         attributes.append((module, kept, False))
         for name in ("site", "site_1", "site_2"):
-            if hasattr(module, name):
-                options = getattr(module, name)
+            options = own.get(name)
+            if isinstance(options, SiteOptions):
                 attributes.append((options, dict(vars(options)), True))
                 attributes.append((options.calib, dict(vars(options.calib)), True))
     shared, last_norm_output = list(_shared), _last_norm_output
