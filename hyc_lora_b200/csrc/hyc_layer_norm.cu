@@ -4,8 +4,8 @@
 //     dz = (g - mean(g) - u * mean(g * u)) * rstd [+ the gradient that reaches z from elsewhere]
 //     dx = keep ? dz / (1 - p) : 0, dresidual = dz, dweight = sum over rows of dy * u, dbias = sum over rows of dy
 // Statistics, sums and gradients are held in fp32; every output is rounded once.  What the dropout keeps is rounded to fp32
-// before the residual is added, as in hyc_dropout.cu.  The forward pass normalises the unrounded
-// sum; the backward pass starts from z as it was stored.
+// before the residual is added, as in hyc_dropout.cu.  The forward pass normalises the unrounded sum; the backward pass starts
+// from z as it was stored.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

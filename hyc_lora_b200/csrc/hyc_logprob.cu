@@ -976,7 +976,7 @@ static int run_logprob(const LogprobArgs& a, int ranks, cudaStream_t stream) {
     cfg.gridDim = dim3(static_cast<unsigned>(clusters * ranks)); cfg.blockDim = dim3(THREADS);
     cfg.stream = stream; cfg.attrs = &attr; cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, kernel, a);
-    cudaGetLastError();                    // a refused launch is this call's error, not also the next one's
+    if (e != cudaSuccess) cudaGetLastError();                    // a refused launch is this call's error, not also the next one's
   } else {
     kernel<<<static_cast<unsigned>(clusters), THREADS, 0, stream>>>(a);
     e = cudaGetLastError();

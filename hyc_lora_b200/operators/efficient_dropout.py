@@ -80,8 +80,7 @@ class EfficientMemoryCounterDropout(torch.nn.Module):
     should differ seeds of their own.  (Under torch's DistributedDataParallel that takes ``broadcast_buffers=False``: by
     default it copies rank 0's buffers, this state among them, to all ranks in front of every forward pass.
     ``hyc_lora_b200.ddp`` exchanges gradients only.)  A forward pass that is run again by activation checkpointing has to see
-    its first mask: take ``rng = module.take()`` outside the checkpointed function
-    and hand it to ``forward``."""
+    its first mask: take ``rng = module.take()`` outside the checkpointed function and hand it to ``forward``."""
 
     def __init__(self, p: float = 0.5, seed=None, device=None):
         super().__init__()
