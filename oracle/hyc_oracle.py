@@ -451,7 +451,8 @@ def linear_backward(x_hat: torch.Tensor, w: torch.Tensor, dy: torch.Tensor):
     autograd engine's reduction of the batched [B,r,D] result to [r,D])."""
     dx = dy.to(w.dtype) @ w
     g = dy.to(x_hat.dtype)
-    dw = (g.transpose(-2, -1) @ x_hat)
+    # summed in 64 bits and rounded once: a library's own product of bf16 matrices differs between CPUs in its last place
+    dw = (g.double().transpose(-2, -1) @ x_hat.double()).to(x_hat.dtype)
     if dw.dim() == 3:
         dw = dw.sum(dim=0)
     return dx, dw.to(w.dtype)
